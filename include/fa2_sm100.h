@@ -69,8 +69,9 @@ enum Fa2Status {
   FA2_ERR_DEVICE = 11,       /* current device is not sm_100 / driver entry point missing */
   FA2_ERR_TIMEOUT = 12,      /* value written to err_flag by a kernel whose bounded wait expired */
   FA2_ERR_WORKSPACE = 13,    /* num_splits > 1 without a large enough, 16-byte aligned workspace */
-  FA2_ERR_SCRATCH_LIMIT = 14 /* fa2_fwd_sm100_noalloc: the split-KV scratch this call needs is
-                                larger than FA2_NOALLOC_SCRATCH_BYTES */
+  FA2_ERR_SCRATCH_LIMIT = 14, /* fa2_fwd_sm100_noalloc: the split-KV scratch this call needs is
+                                 larger than FA2_NOALLOC_SCRATCH_BYTES */
+  FA2_ERR_PAGE = 15           /* err_flag (fa2_kvcache_sm100.h): a block table entry outside the cache */
 };
 /* Device-side reports in err_flag: the kernel writes FA2_ERR_TIMEOUT (a bounded wait expired)
  * or FA2_ERR_SHAPE (a variable-length or paged sequence longer than seqlen_q / seqlen_kv, or

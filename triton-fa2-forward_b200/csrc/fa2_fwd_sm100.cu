@@ -2059,6 +2059,7 @@ const char* fa2_sm100_strerror(int status) {
     case FA2_ERR_TIMEOUT: return "a bounded wait inside the kernel expired";
     case FA2_ERR_WORKSPACE: return "num_splits > 1 needs a 16-byte aligned workspace of fa2_fwd_sm100_workspace_bytes() bytes";
     case FA2_ERR_SCRATCH_LIMIT: return "fa2_fwd_sm100_noalloc: this call needs more split-KV scratch than the library's 32 MiB static array; use fewer splits or fa2_fwd_sm100 with a workspace";
+    case FA2_ERR_PAGE: return "a block table entry of a sequence lies outside the cache";
     default: return "unknown fa2_sm100 status";
   }
 }

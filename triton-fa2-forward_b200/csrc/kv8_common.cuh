@@ -1,0 +1,163 @@
+// Shared pieces of the serving kernels (rotary positions, 8-bit paged K/V cache): page arithmetic,
+// e4m3 conversions, error reports, and the host's checks of a cache.
+#pragma once
+
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "fa2_kvcache_sm100.h"
+
+namespace fa2kv {
+
+constexpr float E4M3_MAX = 448.0f;
+
+// One tensor of codes or scales on the device side.
+struct Cache {
+  const uint8_t* k;
+  const uint8_t* v;
+  const float* ks;
+  const float* vs;
+  int64_t k_st[3], v_st[3], ks_st[3], vs_st[3];  // (page, row, head)
+  int num_pages, page_size, page_shift;           // shift >= 0 where page_size is a power of two
+  int heads_kv;
+};
+
+__device__ __forceinline__ int page_of(const Cache& c, int pos) {
+  return c.page_shift >= 0 ? pos >> c.page_shift : pos / c.page_size;
+}
+
+__device__ __forceinline__ void report(int* err, int code) {
+  if (err != nullptr) atomicCAS(err, 0, code);  // the first report wins
+}
+
+// Two values to two e4m3 codes (low byte: lo), round to nearest even, saturated at +-448.
+__device__ __forceinline__ uint16_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Two e4m3 codes to fp16 (exact: fp16 holds every e4m3 value).
+__device__ __forceinline__ uint32_t f16x2_of_e4m3x2(uint16_t c) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(c));
+  return r;
+}
+
+__device__ __forceinline__ float2 float2_of_f16x2(uint32_t h) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+template <bool BF16>
+__device__ __forceinline__ float2 float2_of_x2(uint32_t w) {
+  if constexpr (BF16) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  } else {
+    return float2_of_f16x2(w);
+  }
+}
+
+template <bool BF16>
+__device__ __forceinline__ float float_of_16(uint16_t w) {
+  if constexpr (BF16) {
+    return __uint_as_float(static_cast<uint32_t>(w) << 16);
+  } else {
+    return __half2float(__ushort_as_half(w));
+  }
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t x2_of_floats(float lo, float hi) {
+  uint32_t r;
+  if constexpr (BF16) {
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  } else {
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  }
+  return r;
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint16_t x1_of_float(float x) {
+  if constexpr (BF16) {
+    return __bfloat16_as_ushort(__float2bfloat16_rn(x));
+  } else {
+    return __half_as_ushort(__float2half_rn(x));
+  }
+}
+
+// The sequence whose packed rows hold row `t`: the largest b with cu[b] <= t among b0.. (cu is
+// non-decreasing where it is right; where it is not, the caller's own range test refuses the row).
+// The block's first row is located by all its threads at once (one round of loads for 256
+// sequences), the others by walking on from there.
+__device__ __forceinline__ int block_first_sequence(const int* cu, int batch, int t) {
+  int n = 0;
+  for (int base = 0; base < batch; base += static_cast<int>(blockDim.x)) {
+    const int i = base + static_cast<int>(threadIdx.x);
+    n += __syncthreads_count(i < batch && __ldg(cu + i + 1) <= t);
+  }
+  return n;
+}
+__device__ __forceinline__ int walk_sequence(const int* cu, int batch, int b, int t) {
+  while (b < batch && __ldg(cu + b + 1) <= t) ++b;
+  return b;
+}
+
+// ------------------------------------------------------------------------------------ host
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+inline bool page_size_ok(int n) { return n == 16 || n == 32 || n == 64 || (n >= 128 && n % 128 == 0); }
+
+inline int check_cache(const Fa2Kv8Cache& c) {
+  if (c.k == nullptr || c.v == nullptr || c.k_scale == nullptr || c.v_scale == nullptr) return FA2_ERR_NULL;
+  if (c.num_pages < 1 || c.heads_kv < 1 || !page_size_ok(c.page_size)) return FA2_ERR_SHAPE;
+  if (c.head_dim != 16 && c.head_dim != 32 && c.head_dim != 64 && c.head_dim != 128) return FA2_ERR_HEAD_DIM;
+  if (!aligned16(c.k) || !aligned16(c.v)) return FA2_ERR_LAYOUT;
+  if ((reinterpret_cast<uintptr_t>(c.k_scale) & 3u) != 0 || (reinterpret_cast<uintptr_t>(c.v_scale) & 3u) != 0) {
+    return FA2_ERR_LAYOUT;
+  }
+  const int64_t n[3] = {c.num_pages, c.page_size, c.heads_kv};
+  for (int i = 0; i < 3; ++i) {
+    if (n[i] > 1 && ((c.k_stride[i] | c.v_stride[i]) & 15) != 0) return FA2_ERR_LAYOUT;
+  }
+  return FA2_OK;
+}
+
+inline Cache device_cache(const Fa2Kv8Cache& c) {
+  Cache d{};
+  d.k = static_cast<const uint8_t*>(c.k);
+  d.v = static_cast<const uint8_t*>(c.v);
+  d.ks = c.k_scale;
+  d.vs = c.v_scale;
+  for (int i = 0; i < 3; ++i) {
+    d.k_st[i] = c.k_stride[i];
+    d.v_st[i] = c.v_stride[i];
+    d.ks_st[i] = c.ks_stride[i];
+    d.vs_st[i] = c.vs_stride[i];
+  }
+  d.num_pages = c.num_pages;
+  d.page_size = c.page_size;
+  d.page_shift = -1;
+  for (int s = 4; s < 31; ++s) {
+    if (c.page_size == (1 << s)) d.page_shift = s;
+  }
+  d.heads_kv = c.heads_kv;
+  return d;
+}
+
+// FA2_OK on an sm_100 device (the current one).
+inline int check_device() {
+  int dev = -1, major = 0, minor = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev) != cudaSuccess) {
+    return FA2_ERR_DEVICE;
+  }
+  return major == 10 && minor == 0 ? FA2_OK : FA2_ERR_DEVICE;
+}
+
+inline int launch_status() { return cudaGetLastError() == cudaSuccess ? FA2_OK : FA2_ERR_LAUNCH; }
+
+}  // namespace fa2kv

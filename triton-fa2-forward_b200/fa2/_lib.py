@@ -33,6 +33,7 @@ FA2_ERR_DEVICE = 11
 FA2_ERR_TIMEOUT = 12
 FA2_ERR_WORKSPACE = 13
 FA2_ERR_SCRATCH_LIMIT = 14
+FA2_ERR_PAGE = 15
 NOALLOC_SCRATCH_BYTES = 32 << 20
 
 # Every symbol the header declares (the ABI test checks the library exports all of them).
