@@ -487,13 +487,21 @@ int check_core(const Fa2Kv8AttnParams* p) {
   return FA2_OK;
 }
 
+// Raises a kernel's shared memory limit, once for each device. `done` is the kernel's own.
+template <typename K>
+bool allow_smem(K kernel, int bytes, int dev, std::atomic<bool> (&done)[MAX_DEVICES]) {
+  if (done[dev].load(std::memory_order_acquire)) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  done[dev].store(true, std::memory_order_release);
+  return true;
+}
+
 template <int D, bool BF16>
-int launch(const AttnArgs& a, cudaStream_t s) {
+int launch(const AttnArgs& a, cudaStream_t s, int dev) {
   static_assert(Dec<D>::SMEM <= 227 * 1024, "shared memory");
+  static std::atomic<bool> done[MAX_DEVICES];
   auto kernel = decode_kernel<D, BF16>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Dec<D>::SMEM) != cudaSuccess) {
-    return FA2_ERR_LAUNCH;
-  }
+  if (!allow_smem(kernel, Dec<D>::SMEM, dev, done)) return FA2_ERR_LAUNCH;
   const int64_t ctas = static_cast<int64_t>(a.batch) * a.heads_kv * a.splits * a.row_blocks;
   kernel<<<static_cast<unsigned>(ctas), DEC_WARPS * 32, Dec<D>::SMEM, s>>>(a);
   int rc = launch_status();
@@ -522,11 +530,11 @@ int64_t fa2_kv8_attn_sm100_workspace_bytes(const Fa2Kv8AttnParams* p) {
 }
 
 int fa2_kv8_attn_sm100(const Fa2Kv8AttnParams* p, void* stream) {
-  int rc = fa2_kv8_attn_sm100_check(p);
+  const int rc = fa2_kv8_attn_sm100_check(p);
   if (rc != FA2_OK) return rc;
   if (p->seqlen_q == 0 || (p->cu_seqlens_q != nullptr && p->total_q == 0)) return FA2_OK;
-  rc = check_device();
-  if (rc != FA2_OK) return rc;
+  const int dev = sm100_device();
+  if (dev < 0) return FA2_ERR_DEVICE;
   const Plan r = plan(p);
   AttnArgs a{};
   a.c = device_cache(p->cache);
@@ -561,10 +569,10 @@ int fa2_kv8_attn_sm100(const Fa2Kv8AttnParams* p, void* stream) {
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf = p->dtype == FA2_DTYPE_BF16;
   switch (p->cache.head_dim) {
-    case 16: return bf ? launch<16, true>(a, s) : launch<16, false>(a, s);
-    case 32: return bf ? launch<32, true>(a, s) : launch<32, false>(a, s);
-    case 64: return bf ? launch<64, true>(a, s) : launch<64, false>(a, s);
-    default: return bf ? launch<128, true>(a, s) : launch<128, false>(a, s);
+    case 16: return bf ? launch<16, true>(a, s, dev) : launch<16, false>(a, s, dev);
+    case 32: return bf ? launch<32, true>(a, s, dev) : launch<32, false>(a, s, dev);
+    case 64: return bf ? launch<64, true>(a, s, dev) : launch<64, false>(a, s, dev);
+    default: return bf ? launch<128, true>(a, s, dev) : launch<128, false>(a, s, dev);
   }
 }
 

@@ -259,10 +259,9 @@ int fa2_kv8_append_sm100_check(const Fa2Kv8AppendParams* p) {
 }
 
 int fa2_kv8_append_sm100(const Fa2Kv8AppendParams* p, void* stream) {
-  int rc = fa2_kv8_append_sm100_check(p);
+  const int rc = fa2_kv8_append_sm100_check(p);
   if (rc != FA2_OK || p->seqlen == 0) return rc;
-  rc = check_device();
-  if (rc != FA2_OK) return rc;
+  if (sm100_device() < 0) return FA2_ERR_DEVICE;
   RowArgs a{};
   a.c = device_cache(p->cache);
   a.x[0] = static_cast<const uint16_t*>(p->k);
@@ -307,10 +306,9 @@ int fa2_kv8_read_sm100_check(const Fa2Kv8ReadParams* p) {
 }
 
 int fa2_kv8_read_sm100(const Fa2Kv8ReadParams* p, void* stream) {
-  int rc = fa2_kv8_read_sm100_check(p);
+  const int rc = fa2_kv8_read_sm100_check(p);
   if (rc != FA2_OK || p->total == 0) return rc;
-  rc = check_device();
-  if (rc != FA2_OK) return rc;
+  if (sm100_device() < 0) return FA2_ERR_DEVICE;
   RowArgs a{};
   a.c = device_cache(p->cache);
   a.x[0] = static_cast<const uint16_t*>(p->k_out);

@@ -2,6 +2,7 @@
 // e4m3 conversions, error reports, and the host's checks of a cache.
 #pragma once
 
+#include <atomic>
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -147,15 +148,25 @@ inline Cache device_cache(const Fa2Kv8Cache& c) {
   return d;
 }
 
-// FA2_OK on an sm_100 device (the current one).
-inline int check_device() {
-  int dev = -1, major = 0, minor = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev) != cudaSuccess) {
-    return FA2_ERR_DEVICE;
+constexpr int MAX_DEVICES = 64;
+
+// The current device, or -1 where it is not an sm_100 one. Each device is asked once: the two
+// attribute queries cost as much as a launch. (Threads that race here write the same value.)
+inline int sm100_device() {
+  static std::atomic<signed char> known[MAX_DEVICES];  // 0: not asked, 1: sm_100, -1: another
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MAX_DEVICES) return -1;
+  signed char k = known[dev].load(std::memory_order_relaxed);
+  if (k == 0) {
+    int major = 0, minor = 0;
+    if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev) != cudaSuccess) {
+      return -1;
+    }
+    k = major == 10 && minor == 0 ? 1 : -1;
+    known[dev].store(k, std::memory_order_relaxed);
   }
-  return major == 10 && minor == 0 ? FA2_OK : FA2_ERR_DEVICE;
+  return k > 0 ? dev : -1;
 }
 
 inline int launch_status() { return cudaGetLastError() == cudaSuccess ? FA2_OK : FA2_ERR_LAUNCH; }

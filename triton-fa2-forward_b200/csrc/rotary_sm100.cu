@@ -201,9 +201,9 @@ int fa2_rotary_sm100_check(const Fa2RotaryParams* p) {
 }
 
 int fa2_rotary_sm100(const Fa2RotaryParams* p, void* stream) {
-  int rc = fa2_rotary_sm100_check(p);
-  if (rc == FA2_OK) rc = check_device();
+  const int rc = fa2_rotary_sm100_check(p);
   if (rc != FA2_OK) return rc;
+  if (sm100_device() < 0) return FA2_ERR_DEVICE;
   RotArgs a{};
   a.x[0] = static_cast<const uint16_t*>(p->q);
   a.x[1] = static_cast<const uint16_t*>(p->k);

@@ -5,6 +5,9 @@ is required; there is no CPU or library fallback.
 
 import ctypes
 import os
+import struct
+
+import torch
 
 from ._lib import Fa2Error, strerror  # noqa: F401  (statuses are shared with the attention library)
 
@@ -31,54 +34,38 @@ EXPORTED = (
 _p, _i32, _i64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
 
 
-class Kv8Cache(ctypes.Structure):
-    """Mirror of `Fa2Kv8Cache`."""
+class Layout:
+    """A parameter struct: its fields' names in order, and the packing of their values (arrays flat).
+    Packed at once into bytes, which costs a call a third of what setting ctypes fields does."""
 
-    _fields_ = [("k", _p), ("v", _p), ("k_scale", _p), ("v_scale", _p),
-                ("k_stride", _i64 * 3), ("v_stride", _i64 * 3), ("ks_stride", _i64 * 3), ("vs_stride", _i64 * 3),
-                ("num_pages", _i32), ("page_size", _i32), ("heads_kv", _i32), ("head_dim", _i32)]
-
-
-class RotaryParams(ctypes.Structure):
-    """Mirror of `Fa2RotaryParams`."""
-
-    _fields_ = [("q", _p), ("k", _p), ("q_out", _p), ("k_out", _p),
-                ("q_stride", _i64 * 4), ("k_stride", _i64 * 4), ("q_out_stride", _i64 * 4), ("k_out_stride", _i64 * 4),
-                ("positions", _p), ("pos_stride", _i64 * 2), ("inv_freq", _p),
-                ("pos_is_64", _i32), ("batch", _i32), ("seqlen", _i32), ("heads_q", _i32), ("heads_kv", _i32),
-                ("head_dim", _i32), ("rotary_dim", _i32), ("dtype", _i32), ("interleaved", _i32), ("inverse", _i32),
-                ("magnitude", ctypes.c_float), ("reserved", _i32)]
+    def __init__(self, *fields):
+        self.fields = [(name, code) for name, code in fields]
+        self.packer = struct.Struct("@" + "".join(code for _, code in fields))
+        self.pack, self.size = self.packer.pack, self.packer.size
 
 
-class AppendParams(ctypes.Structure):
-    """Mirror of `Fa2Kv8AppendParams`."""
+# Native alignment and sizes, as the C compiler lays the structs out. CACHE is the head of three.
+CACHE = (("k", "P"), ("v", "P"), ("k_scale", "P"), ("v_scale", "P"), ("k_stride", "3q"), ("v_stride", "3q"),
+         ("ks_stride", "3q"), ("vs_stride", "3q"), ("num_pages", "i"), ("page_size", "i"), ("heads_kv", "i"),
+         ("head_dim", "i"))
+ROTARY = Layout(("q", "P"), ("k", "P"), ("q_out", "P"), ("k_out", "P"), ("q_stride", "4q"), ("k_stride", "4q"),
+                ("q_out_stride", "4q"), ("k_out_stride", "4q"), ("positions", "P"), ("pos_stride", "2q"),
+                ("inv_freq", "P"), ("pos_is_64", "i"), ("batch", "i"), ("seqlen", "i"), ("heads_q", "i"),
+                ("heads_kv", "i"), ("head_dim", "i"), ("rotary_dim", "i"), ("dtype", "i"), ("interleaved", "i"),
+                ("inverse", "i"), ("magnitude", "f"), ("reserved", "i"))
+APPEND = Layout(*CACHE, ("k_in", "P"), ("v_in", "P"), ("k_in_stride", "4q"), ("v_in_stride", "4q"),
+                ("block_table", "P"), ("cache_seqlens", "P"), ("cu_seqlens", "P"), ("err_flag", "P"),
+                ("block_table_stride", "q"), ("pages_per_seq", "i"), ("batch", "i"), ("seqlen", "i"), ("dtype", "i"))
+READ = Layout(*CACHE, ("k_out", "P"), ("v_out", "P"), ("block_table", "P"), ("cu_seqlens", "P"), ("err_flag", "P"),
+              ("block_table_stride", "q"), ("pages_per_seq", "i"), ("batch", "i"), ("total", "i"), ("dtype", "i"))
+ATTN = Layout(*CACHE, ("q", "P"), ("o", "P"), ("q_stride", "4q"), ("o_stride", "4q"), ("block_table", "P"),
+              ("cache_seqlens", "P"), ("cu_seqlens_q", "P"), ("err_flag", "P"), ("workspace", "P"),
+              ("workspace_bytes", "q"), ("block_table_stride", "q"), ("timeout_cycles", "q"), ("pages_per_seq", "i"),
+              ("batch", "i"), ("heads_q", "i"), ("seqlen_q", "i"), ("total_q", "i"), ("max_seqlen_k", "i"),
+              ("dtype", "i"), ("causal", "i"), ("causal_align", "i"), ("num_splits", "i"), ("qk_scale", "f"),
+              ("reserved", "i"))
 
-    _fields_ = [("cache", Kv8Cache), ("k", _p), ("v", _p), ("k_in_stride", _i64 * 4), ("v_in_stride", _i64 * 4),
-                ("block_table", _p), ("cache_seqlens", _p), ("cu_seqlens", _p), ("err_flag", _p),
-                ("block_table_stride", _i64), ("pages_per_seq", _i32), ("batch", _i32), ("seqlen", _i32),
-                ("dtype", _i32)]
-
-
-class ReadParams(ctypes.Structure):
-    """Mirror of `Fa2Kv8ReadParams`."""
-
-    _fields_ = [("cache", Kv8Cache), ("k_out", _p), ("v_out", _p), ("block_table", _p), ("cu_seqlens", _p),
-                ("err_flag", _p), ("block_table_stride", _i64), ("pages_per_seq", _i32), ("batch", _i32),
-                ("total", _i32), ("dtype", _i32)]
-
-
-class AttnParams(ctypes.Structure):
-    """Mirror of `Fa2Kv8AttnParams`."""
-
-    _fields_ = [("cache", Kv8Cache), ("q", _p), ("o", _p), ("q_stride", _i64 * 4), ("o_stride", _i64 * 4),
-                ("block_table", _p), ("cache_seqlens", _p), ("cu_seqlens_q", _p), ("err_flag", _p),
-                ("workspace", _p), ("workspace_bytes", _i64), ("block_table_stride", _i64), ("timeout_cycles", _i64),
-                ("pages_per_seq", _i32), ("batch", _i32), ("heads_q", _i32), ("seqlen_q", _i32), ("total_q", _i32),
-                ("max_seqlen_k", _i32), ("dtype", _i32), ("causal", _i32), ("causal_align", _i32),
-                ("num_splits", _i32), ("qk_scale", ctypes.c_float), ("reserved", _i32)]
-
-
-STRUCTS = (RotaryParams, AppendParams, ReadParams, AttnParams)
+STRUCTS = (ROTARY, APPEND, READ, ATTN)  # the order of fa2_kvcache_sm100_params_size
 _lib = None
 
 
@@ -94,25 +81,28 @@ def lib():
     L.fa2_kvcache_sm100_abi_version.restype = ctypes.c_int
     L.fa2_kvcache_sm100_params_size.argtypes = [_i32]
     L.fa2_kvcache_sm100_params_size.restype = _i64
-    for name, struct in (("fa2_rotary_sm100", RotaryParams), ("fa2_kv8_append_sm100", AppendParams),
-                         ("fa2_kv8_read_sm100", ReadParams), ("fa2_kv8_attn_sm100", AttnParams)):
+    for name in ("fa2_rotary_sm100", "fa2_kv8_append_sm100", "fa2_kv8_read_sm100", "fa2_kv8_attn_sm100"):
         f, check = getattr(L, name), getattr(L, name + "_check")
-        f.argtypes, f.restype = [ctypes.POINTER(struct), _p], ctypes.c_int
-        check.argtypes, check.restype = [ctypes.POINTER(struct)], ctypes.c_int
-    L.fa2_kv8_attn_sm100_workspace_bytes.argtypes = [ctypes.POINTER(AttnParams)]
+        f.argtypes, f.restype = [ctypes.c_char_p, _p], ctypes.c_int  # the packed struct, read only
+        check.argtypes, check.restype = [ctypes.c_char_p], ctypes.c_int
+    L.fa2_kv8_attn_sm100_workspace_bytes.argtypes = [ctypes.c_char_p]
     L.fa2_kv8_attn_sm100_workspace_bytes.restype = _i64
     if L.fa2_kvcache_sm100_abi_version() != ABI_VERSION:
         raise ImportError(f"{LIB_PATH}: ABI version {L.fa2_kvcache_sm100_abi_version()} != {ABI_VERSION}")
-    for i, struct in enumerate(STRUCTS):
-        if L.fa2_kvcache_sm100_params_size(i) != ctypes.sizeof(struct):
-            raise ImportError(f"{LIB_PATH}: size of {struct.__name__} {L.fa2_kvcache_sm100_params_size(i)} != "
-                              f"ctypes mirror {ctypes.sizeof(struct)}")
+    for i, layout in enumerate(STRUCTS):
+        if L.fa2_kvcache_sm100_params_size(i) != layout.size:
+            raise ImportError(f"{LIB_PATH}: size of struct {i} {L.fa2_kvcache_sm100_params_size(i)} != {layout.size} packed")
     _lib = L
     return L
 
 
-def launch(name, params, stream_handle):
-    """Runs one entry point; raises Fa2Error for a status other than OK."""
-    rc = getattr(lib(), name)(ctypes.byref(params), _p(stream_handle or None))
+def launch(entry, packed, index):
+    """Runs one entry point of lib() on torch's current stream of CUDA device `index`; raises
+    Fa2Error for a status other than OK."""
+    if index == torch.cuda.current_device():
+        rc = entry(packed, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = entry(packed, torch._C._cuda_getCurrentRawStream(index))
     if rc != 0:
         raise Fa2Error(rc, strerror(rc))

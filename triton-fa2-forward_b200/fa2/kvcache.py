@@ -24,6 +24,9 @@ from . import _kvlib, _lib
 from .kernel import CAUSAL_ALIGNS, LOG2E, _err_word, _sync_check_enabled, check_device_errors
 
 
+_DTYPES = (torch.float16, torch.bfloat16)
+
+
 class KVCacheFP8(NamedTuple):
     """k, v: float8_e4m3fn [num_pages, page_size, H_kv, D]; k_scale, v_scale: float32
     [num_pages, page_size, H_kv]. Any strides with adjacent D values on 16-byte boundaries; any
@@ -46,69 +49,70 @@ def alloc_kvcache_fp8(num_pages, page_size, heads_kv, head_dim, device=None):
     return KVCacheFP8(*made)
 
 
-def _check_cache(cache):
+def _cache_fields(cache):
+    """The cache's part of a parameter struct, its [H_kv, D], and its tensors; checked."""
     assert len(cache) == 4, "cache must be (k, v, k_scale, v_scale)"
     k, v, ks, vs = cache
-    assert k.dim() == 4 and v.shape == k.shape, "cache k and v must be [num_pages, page_size, H_kv, D]"
+    shape = k.shape
+    assert len(shape) == 4 and v.shape == shape, "cache k and v must be [num_pages, page_size, H_kv, D]"
     assert k.dtype == v.dtype == torch.float8_e4m3fn, "cache codes must be float8_e4m3fn"
-    assert ks.shape == vs.shape == k.shape[:3], "cache scales must be [num_pages, page_size, H_kv]"
+    pages, page_size, H_kv, D = shape
+    assert ks.shape == vs.shape == (pages, page_size, H_kv), "cache scales must be [num_pages, page_size, H_kv]"
     assert ks.dtype == vs.dtype == torch.float32, "cache scales must be float32"
-    assert k.shape[3] in (16, 32, 64, 128), "head_dim must be a power of two in [16, 128]"
-    page_size = k.shape[1]
+    assert D in (16, 32, 64, 128), "head_dim must be a power of two in [16, 128]"
     assert page_size in (16, 32, 64) or (page_size >= 128 and page_size % 128 == 0), "page_size"
-    assert k.shape[0] > 0 and k.shape[2] > 0, "the cache has no pages or no heads"
-    return k, v, ks, vs
-
-
-def _fill_cache(c, cache):
-    k, v, ks, vs = cache
-    c.k, c.v, c.k_scale, c.v_scale = k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()
-    if k.stride(3) != 1 or v.stride(3) != 1:
+    assert pages > 0 and H_kv > 0, "the cache has no pages or no heads"
+    k_st, v_st = k.stride(), v.stride()
+    if k_st[3] != 1 or v_st[3] != 1:
         raise _lib.Fa2Error(_lib.FA2_ERR_LAYOUT, "the D values of a cache row must be adjacent")
-    c.k_stride[:], c.v_stride[:] = k.stride()[:3], v.stride()[:3]
-    c.ks_stride[:], c.vs_stride[:] = ks.stride(), vs.stride()
-    c.num_pages, c.page_size, c.heads_kv, c.head_dim = k.shape
+    fields = (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), *k_st[:3], *v_st[:3], *ks.stride(), *vs.stride(),
+              pages, page_size, H_kv, D)
+    return fields, shape, cache
 
 
-def _check_table(name, block_table, B, *lengths):
-    assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == B, \
+def _check_table(block_table, *lengths):
+    """B of a block table [B, pages_per_seq]; `lengths`: (tensor, entries more than B)."""
+    shape = block_table.shape
+    assert block_table.dtype == torch.int32 and len(shape) == 2 and shape[0] > 0, \
         "block_table must be int32 [B, pages_per_seq]"
-    for t, n in lengths:
-        assert t.dtype == torch.int32 and t.shape == (n,), "sequence lengths and their sums must be int32"
+    for t, more in lengths:
+        assert t.dtype == torch.int32 and t.shape == (shape[0] + more,), \
+            "cache_seqlens must be int32 [B], cu_seqlens int32 [B + 1], B as in block_table"
+    return shape[0]
 
 
-def _check_devices(name, *tensors):
-    if not all(t.is_cuda for t in tensors):
-        raise RuntimeError(f"fa2.kvcache.{name} runs only on an sm_100 CUDA device (no CPU path)")
-    if not all(t.device == tensors[0].device for t in tensors):
-        raise RuntimeError(f"fa2.kvcache.{name}: all tensors must be on the same CUDA device")
+def _check_device(name, *tensors):
+    """The index of the one CUDA device that holds the tensors."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        at = t.get_device()
+        if at < 0 or index < 0:
+            raise RuntimeError(f"fa2.kvcache.{name} runs only on an sm_100 CUDA device (no CPU path)")
+        if at != index:
+            raise RuntimeError(f"fa2.kvcache.{name}: all tensors must be on the same CUDA device")
+    return index
 
 
 def _no_grad(name, *tensors):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError(f"fa2.kvcache.{name} is forward only: use it under torch.no_grad()")
+    for t in tensors:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"fa2.kvcache.{name} is forward only: use it under torch.no_grad()")
 
 
 def _rows(t):
     """(b, h, n, d) strides of [B, H, N, D] or of packed [total, H, D]."""
-    if t.dim() == 4:
-        return tuple(int(s) for s in t.stride())
-    return (0, int(t.stride(1)), int(t.stride(0)), int(t.stride(2)))
+    st = t.stride()
+    return st if len(st) == 4 else (0, st[1], st[0], st[2])
 
 
 def _table(block_table):
     return block_table if block_table.stride(1) == 1 or block_table.shape[1] <= 1 else block_table.contiguous()
 
 
-def _dtype(t):
-    return _lib.FA2_DTYPE_BF16 if t == torch.bfloat16 else _lib.FA2_DTYPE_FP16
-
-
-def _run(name, p, device):
-    with torch.cuda.device(device):
-        _kvlib.launch(name, p, torch.cuda.current_stream(device).cuda_stream)
-        if _sync_check_enabled():
-            check_device_errors(device)
+def _launch(entry, packed, index):
+    _kvlib.launch(entry, packed, index)
+    if _sync_check_enabled():
+        check_device_errors(torch.device("cuda", index))
 
 
 def kvcache_append_fp8(k, v, cache, block_table, cache_seqlens, cu_seqlens=None):
@@ -121,32 +125,30 @@ def kvcache_append_fp8(k, v, cache, block_table, cache_seqlens, cu_seqlens=None)
     [B, pages_per_seq]. Two sequences that share a page may both read it, but the rows that one call
     writes must be distinct. Returns the cache; asynchronous on torch's current stream.
     """
-    ck, cv, cks, cvs = _check_cache(cache)
-    assert k.dim() == (4 if cu_seqlens is None else 3) and v.shape == k.shape, \
+    fields, shape, tensors = _cache_fields(cache)
+    k_shape, dtype = k.shape, k.dtype
+    assert len(k_shape) == (4 if cu_seqlens is None else 3) and v.shape == k_shape, \
         "k and v must be [B, H_kv, N, D], or [total, H_kv, D] with cu_seqlens"
-    assert k.dtype == v.dtype and k.dtype in (torch.float16, torch.bfloat16)
-    assert tuple(k.shape[-1:]) == tuple(ck.shape[3:]) and k.shape[1] == ck.shape[2], "k must have the cache's heads and D"
-    B = block_table.shape[0] if block_table.dim() else 0
-    assert B > 0, "block_table must be int32 [B, pages_per_seq]"
-    _check_table("kvcache_append_fp8", block_table, B, (cache_seqlens, B),
-                 *([(cu_seqlens, B + 1)] if cu_seqlens is not None else []))
-    assert cu_seqlens is not None or k.shape[0] == B, "k's batch must be block_table's"
-    _check_devices("kvcache_append_fp8", k, v, ck, cv, cks, cvs, block_table, cache_seqlens,
-                   *([cu_seqlens] if cu_seqlens is not None else []))
+    assert dtype in _DTYPES and v.dtype == dtype, "k and v must be fp16 or bf16"
+    assert k_shape[-1] == shape[3] and k_shape[1] == shape[2], "k and v must have the cache's H_kv and D"
+    if cu_seqlens is None:
+        B = _check_table(block_table, (cache_seqlens, 0))
+        assert k_shape[0] == B, "k and v must have block_table's batch"
+        index = _check_device("kvcache_append_fp8", k, v, *tensors, block_table, cache_seqlens)
+        cu, n = 0, k_shape[2]
+    else:
+        B = _check_table(block_table, (cache_seqlens, 0), (cu_seqlens, 1))
+        index = _check_device("kvcache_append_fp8", k, v, *tensors, block_table, cache_seqlens, cu_seqlens)
+        cu_seqlens = cu_seqlens.contiguous()
+        cu, n = cu_seqlens.data_ptr(), k_shape[0]
     _no_grad("kvcache_append_fp8", k, v)
-    if k.numel() == 0:
+    if n == 0:
         return cache
     bt, sl = _table(block_table), cache_seqlens.contiguous()
-    cu = cu_seqlens.contiguous() if cu_seqlens is not None else None
-    p = _kvlib.AppendParams()
-    _fill_cache(p.cache, (ck, cv, cks, cvs))
-    p.k, p.v = k.data_ptr(), v.data_ptr()
-    p.k_in_stride[:], p.v_in_stride[:] = _rows(k), _rows(v)
-    p.block_table, p.cache_seqlens, p.err_flag = bt.data_ptr(), sl.data_ptr(), _err_word(k.device).data_ptr()
-    p.cu_seqlens = cu.data_ptr() if cu is not None else None
-    p.block_table_stride, p.pages_per_seq = bt.stride(0), bt.shape[1]
-    p.batch, p.seqlen, p.dtype = B, k.shape[2] if cu is None else k.shape[0], _dtype(k.dtype)
-    _run("fa2_kv8_append_sm100", p, k.device)
+    packed = _kvlib.APPEND.pack(
+        *fields, k.data_ptr(), v.data_ptr(), *_rows(k), *_rows(v), bt.data_ptr(), sl.data_ptr(), cu,
+        _err_word(k.device).data_ptr(), bt.stride(0), bt.shape[1], B, n, dtype == torch.bfloat16)
+    _launch(_kvlib.lib().fa2_kv8_append_sm100, packed, index)
     return cache
 
 
@@ -155,25 +157,22 @@ def kvcache_read_fp8(cache, block_table, cu_seqlens, total, dtype=torch.bfloat16
     16 bits and packed as attention_varlen takes them: (k, v), each [total, H_kv, D]. Rows past
     cu_seqlens[B] are not written; rows of a refused page are zeros. Asynchronous.
     """
-    ck, cv, cks, cvs = _check_cache(cache)
-    assert dtype in (torch.float16, torch.bfloat16)
-    assert block_table.dim() == 2 and block_table.shape[0] > 0, "block_table must be int32 [B, pages_per_seq]"
-    B = block_table.shape[0]
-    _check_table("kvcache_read_fp8", block_table, B, (cu_seqlens, B + 1))
+    fields, shape, tensors = _cache_fields(cache)
+    assert dtype in _DTYPES, "dtype must be fp16 or bf16"
+    B = _check_table(block_table, (cu_seqlens, 1))
+    total = int(total)
     assert total >= 0, "total must not be negative"
-    _check_devices("kvcache_read_fp8", ck, cv, cks, cvs, block_table, cu_seqlens)
-    shape = (int(total), ck.shape[2], ck.shape[3])
-    k, v = (torch.empty(shape, dtype=dtype, device=ck.device) for _ in range(2))
+    index = _check_device("kvcache_read_fp8", *tensors, block_table, cu_seqlens)
+    device = tensors[0].device
+    k = torch.empty((total, shape[2], shape[3]), dtype=dtype, device=device)
+    v = torch.empty_like(k)
     if total == 0:
         return k, v
     bt, cu = _table(block_table), cu_seqlens.contiguous()
-    p = _kvlib.ReadParams()
-    _fill_cache(p.cache, (ck, cv, cks, cvs))
-    p.k_out, p.v_out = k.data_ptr(), v.data_ptr()
-    p.block_table, p.cu_seqlens, p.err_flag = bt.data_ptr(), cu.data_ptr(), _err_word(ck.device).data_ptr()
-    p.block_table_stride, p.pages_per_seq = bt.stride(0), bt.shape[1]
-    p.batch, p.total, p.dtype = B, int(total), _dtype(dtype)
-    _run("fa2_kv8_read_sm100", p, ck.device)
+    packed = _kvlib.READ.pack(
+        *fields, k.data_ptr(), v.data_ptr(), bt.data_ptr(), cu.data_ptr(), _err_word(device).data_ptr(),
+        bt.stride(0), bt.shape[1], B, total, dtype == torch.bfloat16)
+    _launch(_kvlib.lib().fa2_kv8_read_sm100, packed, index)
     return k, v
 
 
@@ -190,69 +189,67 @@ def attention_kvcache_fp8(q, cache, block_table, cache_seqlens, max_seqlen_k=Non
     another (None: chosen from the sizes). A query that sees a key of a refused page gets NaN. Returns
     a tensor like q (rows past cu_seqlens_q[B] are not written), asynchronously.
     """
-    ck, cv, cks, cvs = _check_cache(cache)
+    fields, shape, tensors = _cache_fields(cache)
+    q_shape, dtype = q.shape, q.dtype
     packed = cu_seqlens_q is not None
-    assert q.dim() == (3 if packed else 4), "q must be [B, H_q, N_q, D], or [total_q, H_q, D] with cu_seqlens_q"
-    assert q.dtype in (torch.float16, torch.bfloat16)
-    H_q, D = q.shape[1], q.shape[-1]
-    H_kv = ck.shape[2]
-    assert D == ck.shape[3], "q must have the cache's head_dim"
+    assert len(q_shape) == (3 if packed else 4), "q must be [B, H_q, N_q, D], or [total_q, H_q, D] with cu_seqlens_q"
+    assert dtype in _DTYPES, "q must be fp16 or bf16"
+    _, page_size, H_kv, D = shape
+    H_q = q_shape[1]
+    assert q_shape[-1] == D, "q must have the cache's head_dim"
     assert H_q % H_kv == 0, "GQA needs H_q divisible by H_kv"
     assert causal_align in CAUSAL_ALIGNS, f"causal_align must be one of {sorted(CAUSAL_ALIGNS)}"
-    assert block_table.dim() == 2 and block_table.shape[0] > 0, "block_table must be int32 [B, pages_per_seq]"
-    B = block_table.shape[0]
-    _check_table("attention_kvcache_fp8", block_table, B, (cache_seqlens, B),
-                 *([(cu_seqlens_q, B + 1)] if packed else []))
     if packed:
+        B = _check_table(block_table, (cache_seqlens, 0), (cu_seqlens_q, 1))
         assert max_seqlen_q is not None and max_seqlen_q >= 0, "packed queries need max_seqlen_q"
         n_q = int(max_seqlen_q)
+        index = _check_device("attention_kvcache_fp8", q, *tensors, block_table, cache_seqlens, cu_seqlens_q)
+        cu_seqlens_q = cu_seqlens_q.contiguous()
     else:
-        assert q.shape[0] == B, "q's batch must be block_table's"
-        n_q = q.shape[2]
+        B = _check_table(block_table, (cache_seqlens, 0))
+        assert q_shape[0] == B, "q must have block_table's batch"
+        n_q = q_shape[2]
+        index = _check_device("attention_kvcache_fp8", q, *tensors, block_table, cache_seqlens)
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(D)
     if not sm_scale > 0:
         raise ValueError(f"sm_scale must be positive (the row max is scaled after it is taken), got {sm_scale}")
-    _check_devices("attention_kvcache_fp8", q, ck, cv, cks, cvs, block_table, cache_seqlens,
-                   *([cu_seqlens_q] if packed else []))
     _no_grad("attention_kvcache_fp8", q)
+    pages_per_seq = block_table.shape[1]
     if max_seqlen_k is None:
-        max_seqlen_k = block_table.shape[1] * ck.shape[1]
+        max_seqlen_k = min(pages_per_seq * page_size, 2 ** 31 - 1)
     out = torch.empty_like(q)
     if out.numel() == 0 or n_q == 0:
         return out
-    if max_seqlen_k == 0 or block_table.shape[1] == 0:
+    if max_seqlen_k == 0 or pages_per_seq == 0:
         return out.zero_()
     bt, sl = _table(block_table), cache_seqlens.contiguous()
-    cu = cu_seqlens_q.contiguous() if packed else None
-    p = _kvlib.AttnParams()
-    _fill_cache(p.cache, (ck, cv, cks, cvs))
-    p.block_table, p.cache_seqlens, p.err_flag = bt.data_ptr(), sl.data_ptr(), _err_word(q.device).data_ptr()
-    p.cu_seqlens_q = cu.data_ptr() if packed else None
-    p.block_table_stride, p.pages_per_seq = bt.stride(0), bt.shape[1]
-    p.batch, p.heads_q, p.seqlen_q, p.total_q = B, H_q, n_q, q.shape[0] if packed else 0
-    p.max_seqlen_k, p.dtype = int(max_seqlen_k), _dtype(q.dtype)
-    p.causal, p.causal_align = int(bool(causal)), CAUSAL_ALIGNS[causal_align]
-    p.num_splits = 0 if num_splits is None else max(1, int(num_splits))
-    p.qk_scale = sm_scale * LOG2E
     qq, oo = q, out
     if not _aligned(q) or not _aligned(out):  # layout copy: rows are moved 16 bytes at a time
         qq = q.clone(memory_format=torch.contiguous_format)
         oo = torch.empty_like(qq)
-    p.q, p.o = qq.data_ptr(), oo.data_ptr()
-    p.q_stride[:], p.o_stride[:] = _rows(qq), _rows(oo)
-    with torch.cuda.device(q.device):
-        nbytes = _kvlib.lib().fa2_kv8_attn_sm100_workspace_bytes(p)
-        ws = torch.empty(max(0, nbytes), dtype=torch.uint8, device=q.device)  # caching allocator, this stream's
-        p.workspace, p.workspace_bytes = ws.data_ptr() if nbytes > 0 else None, max(0, nbytes)
-        _kvlib.launch("fa2_kv8_attn_sm100", p, torch.cuda.current_stream(q.device).cuda_stream)
-        if oo is not out:
-            out.copy_(oo)
-        if _sync_check_enabled():
-            check_device_errors(q.device)
+    L = _kvlib.lib()
+    head = (*fields, qq.data_ptr(), oo.data_ptr(), *_rows(qq), *_rows(oo), bt.data_ptr(), sl.data_ptr(),
+            cu_seqlens_q.data_ptr() if packed else 0, _err_word(q.device).data_ptr())
+    tail = (bt.stride(0), 0, pages_per_seq, B, H_q, n_q, q_shape[0] if packed else 0, int(max_seqlen_k),
+            dtype == torch.bfloat16, bool(causal), CAUSAL_ALIGNS[causal_align],
+            0 if num_splits is None else max(1, int(num_splits)), sm_scale * LOG2E, 0)
+    call = _kvlib.ATTN.pack(*head, 0, 0, *tail)
+    nbytes = L.fa2_kv8_attn_sm100_workspace_bytes(call)
+    if nbytes > 0:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)  # caching allocator, this stream's
+        call = _kvlib.ATTN.pack(*head, ws.data_ptr(), nbytes, *tail)
+    _launch(L.fa2_kv8_attn_sm100, call, index)
+    if oo is not out:
+        out.copy_(oo)
     return out
 
 
 def _aligned(t):
-    return t.data_ptr() % 16 == 0 and t.stride(-1) == 1 and all(
-        n <= 1 or s % 8 == 0 for n, s in zip(t.shape[:-1], t.stride()[:-1]))
+    *st, inner = t.stride()
+    if t.data_ptr() % 16 or inner != 1:
+        return False
+    for n, s in zip(t.shape, st):
+        if s % 8 and n > 1:
+            return False
+    return True

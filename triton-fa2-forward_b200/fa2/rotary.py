@@ -11,7 +11,7 @@ import math
 
 import torch
 
-from . import _kvlib, _lib
+from . import _kvlib
 
 SCALINGS = (None, "linear", "ntk", "yarn")
 
@@ -52,10 +52,13 @@ def rotary_inv_freq(rotary_dim, base=10000.0, scaling=None, factor=1.0, original
     return f.to(device), magnitude
 
 
+_DTYPES = (torch.float16, torch.bfloat16)  # the index is the C ABI's Fa2DType
+_NONE = (0, 0, 0, 0)
+
+
 def _strides4(t):
-    if t.dim() == 4:
-        return tuple(int(s) for s in t.stride())
-    return (0, int(t.stride(1)), int(t.stride(0)), int(t.stride(2)))  # [total, H, D]
+    st = t.stride()
+    return st if len(st) == 4 else (0, st[1], st[0], st[2])  # [total, H, D]
 
 
 def _overlaps(t):
@@ -75,59 +78,60 @@ def rotary(q, k, positions, inv_freq, interleaved=False, inverse=False, magnitud
     map. inplace=True writes into q and k themselves. Returns (q', k'); k' is None where k is.
     Asynchronous on torch's current stream.
     """
-    assert q.dim() in (3, 4), "q must be [B, H, N, D] or [total, H, D]"
-    assert q.dtype in (torch.float16, torch.bfloat16)
-    if q.dim() == 4:
-        B, H_q, N, D = q.shape
-        assert positions.shape in ((B, N), (N,)), "positions must be [B, N] or [N]"
-        pos_stride = (int(positions.stride(0)) if positions.dim() == 2 else 0, int(positions.stride(-1)))
+    dims, dtype = q.dim(), q.dtype
+    assert dims in (3, 4), "q must be [B, H, N, D] or [total, H, D]"
+    assert dtype in _DTYPES, "q must be fp16 or bf16"
+    q_shape, pos_shape = q.shape, positions.shape
+    pos_st = positions.stride()
+    if dims == 4:
+        B, H_q, N, D = q_shape
+        assert pos_shape == (B, N) or pos_shape == (N,), "positions must be [B, N] or [N]"
+        if len(pos_st) == 1:
+            pos_st = (0, *pos_st)
     else:
-        B, (N, H_q, D) = 1, q.shape
-        assert positions.shape == (N,), "positions must be [total]"
-        pos_stride = (0, int(positions.stride(0)))
+        B, (N, H_q, D) = 1, q_shape
+        assert pos_shape == (N,), "positions must be [total]"
+        pos_st = (0, *pos_st)
+    H_kv = 0
     if k is not None:
-        want = (B, k.shape[1], N, D) if q.dim() == 4 else (N, k.shape[1], D)
-        assert k.dim() == q.dim() and tuple(k.shape) == want and k.dtype == q.dtype, "k must match q"
-    assert positions.dtype in (torch.int32, torch.int64)
-    assert inv_freq.dtype == torch.float64 and inv_freq.dim() == 1
+        k_shape = k.shape
+        H_kv = k_shape[1] if len(k_shape) > 1 else 0
+        assert k.dtype == dtype and k_shape == ((B, H_kv, N, D) if dims == 4 else (N, H_kv, D)), "k must match q"
+    pos_dtype = positions.dtype
+    assert pos_dtype == torch.int64 or pos_dtype == torch.int32, "positions must be int32 or int64"
+    assert inv_freq.dtype == torch.float64 and inv_freq.dim() == 1, "inv_freq must be float64 [rotary_dim / 2]"
     rd = 2 * inv_freq.numel()
     assert 2 <= rd <= D, "inv_freq must have between 1 and D / 2 entries"
     if not 0 < magnitude < 3e38:
         raise ValueError(f"magnitude must be positive and finite, got {magnitude}")
-    tensors = [t for t in (q, k, positions, inv_freq) if t is not None]
-    if not all(t.is_cuda for t in tensors):
+    index = q.get_device()  # -1: not on CUDA
+    if index < 0 or positions.get_device() < 0 or inv_freq.get_device() < 0 or (k is not None and k.get_device() < 0):
         raise RuntimeError("fa2.rotary.rotary runs only on an sm_100 CUDA device (no CPU path)")
-    if not all(t.device == q.device for t in tensors):
+    if positions.get_device() != index or inv_freq.get_device() != index or (k is not None and k.get_device() != index):
         raise RuntimeError("q, k, positions and inv_freq must be on the same CUDA device")
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
         raise RuntimeError("fa2.rotary.rotary is forward only: use it under torch.no_grad(); "
                            "inverse=True gives the gradient")
+    if k is not None and H_kv == 0:
+        raise ValueError("k has no heads: pass None")
     if inplace:
         if _overlaps(q) or (k is not None and _overlaps(k)):
             raise ValueError("inplace needs tensors whose values do not share memory (no expanded dimensions)")
         q_out, k_out = q, k
     else:
         q_out, k_out = torch.empty_like(q), None if k is None else torch.empty_like(k)
-    if q.numel() == 0:
-        if k is not None and k.numel() and not inplace:
-            raise ValueError("q has no values but k does")
+    if B == 0 or N == 0:
         return q_out, k_out
-    if k is not None and k.numel() == 0:
-        raise ValueError("k has no heads: pass None")
-    freq = inv_freq.contiguous()
-    p = _kvlib.RotaryParams()
-    p.q, p.q_out = q.data_ptr(), q_out.data_ptr()
-    p.q_stride[:], p.q_out_stride[:] = _strides4(q), _strides4(q_out)
-    if k is not None:
-        p.k, p.k_out = k.data_ptr(), k_out.data_ptr()
-        p.k_stride[:], p.k_out_stride[:] = _strides4(k), _strides4(k_out)
-    p.positions, p.inv_freq = positions.data_ptr(), freq.data_ptr()
-    p.pos_stride[:] = pos_stride
-    p.pos_is_64 = int(positions.dtype == torch.int64)
-    p.batch, p.seqlen, p.heads_q, p.heads_kv = B, N, H_q, 0 if k is None else k.shape[1]
-    p.head_dim, p.rotary_dim = D, rd
-    p.dtype = _lib.FA2_DTYPE_BF16 if q.dtype == torch.bfloat16 else _lib.FA2_DTYPE_FP16
-    p.interleaved, p.inverse, p.magnitude = int(bool(interleaved)), int(bool(inverse)), float(magnitude)
-    with torch.cuda.device(q.device):
-        _kvlib.launch("fa2_rotary_sm100", p, torch.cuda.current_stream(q.device).cuda_stream)
+    if H_q == 0:
+        raise ValueError("q has no heads")
+    if inv_freq.stride(0) != 1:
+        inv_freq = inv_freq.contiguous()
+    packed = _kvlib.ROTARY.pack(
+        q.data_ptr(), 0 if k is None else k.data_ptr(), q_out.data_ptr(), 0 if k is None else k_out.data_ptr(),
+        *_strides4(q), *(_NONE if k is None else _strides4(k)),
+        *_strides4(q_out), *(_NONE if k is None else _strides4(k_out)),
+        positions.data_ptr(), *pos_st, inv_freq.data_ptr(),
+        pos_dtype == torch.int64, B, N, H_q, H_kv, D, rd, dtype == torch.bfloat16,
+        bool(interleaved), bool(inverse), magnitude, 0)
+    _kvlib.launch(_kvlib.lib().fa2_rotary_sm100, packed, index)
     return q_out, k_out
