@@ -205,10 +205,14 @@ def tolerance(q, weight, spread, out, n, v_top):
     have it. P' = p sv 2^k is rounded to fp16: 2^-11, or 2^-31 of the largest |v| for a subnormal
     one, n of them at most. The fp32 sums over n keys: n / 8 * 2^-23 each. The output is rounded
     once: eps / 2, half a subnormal step at the bottom of fp16. What an element is off by is relative
-    to weight = sum p |v| / sum p."""
+    to weight = sum p |v| / sum p.
+
+    bf16 queries of many rows run on code * scale rounded to fp16 (half a step: 2^-11): a score is
+    off by 2^-11 spread more (log2(e) and ln(2) cancel), a value by 2^-11 of itself."""
     D = q.shape[-1]
-    dx = (D + 8) * 2.0 ** -23 * spread[..., None] + 2.0 ** -22
-    rel = 2.0 ** -11 + 2 * dx + 2 * n / 8 * 2.0 ** -23
+    folded = 2.0 ** -11 if q.dtype == torch.bfloat16 else 0.0
+    dx = ((D + 8) * 2.0 ** -23 + folded) * spread[..., None] + 2.0 ** -22
+    rel = 2.0 ** -11 + folded + 2 * dx + 2 * n / 8 * 2.0 ** -23
     eps = torch.finfo(q.dtype).eps / 2
     return weight * rel * (1 + eps) + eps * out.abs() + n * 2.0 ** -31 * v_top + SUBNORMAL[q.dtype]
 

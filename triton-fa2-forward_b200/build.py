@@ -28,7 +28,7 @@ DEPENDS = SOURCES + [
 
 KV_LIB_PATH = os.path.join(PKG_DIR, "fa2", "libfa2_kvcache_sm100.so")
 KV_SOURCES = [os.path.join(CSRC, f) for f in ("rotary_sm100.cu", "kv8_cache_sm100.cu", "kv8_attn_sm100.cu")]
-KV_DEPENDS = KV_SOURCES + [os.path.join(CSRC, f) for f in ("kv8_common.cuh", "kv8_attn.cuh", "ptx_sm100.cuh")] + [
+KV_DEPENDS = KV_SOURCES + [os.path.join(CSRC, f) for f in ("kv8_common.cuh", "kv8_attn.cuh", "kv8_chunk.cuh", "ptx_sm100.cuh")] + [
     os.path.join(INCLUDE, "fa2_sm100.h"),
     os.path.join(INCLUDE, "fa2_kvcache_sm100.h"),
 ]

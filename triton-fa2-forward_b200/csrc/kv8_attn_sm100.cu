@@ -1,6 +1,7 @@
 // Attention of new tokens over the 8-bit paged cache, for sm_100a.
 
 #include "kv8_attn.cuh"
+#include "kv8_chunk.cuh"
 
 #include <cmath>
 
@@ -429,27 +430,35 @@ __global__ void __launch_bounds__(128) merge_kernel(const AttnArgs a) {
 
 // ------------------------------------------------------------------------------------ host
 struct Plan {
+  bool chunk = false;  // the 256-row kernel
   int row_blocks = 1, rows_pad = 16, splits = 1, split_keys = 0;
   int64_t lse_floats = 0, bytes = 0;
 };
 
 constexpr int MAX_SPLITS = 256;
 
+// The kernel and the key ranges of a call, from its sizes alone.
 Plan plan(const Fa2Kv8AttnParams* p) {
   Plan r;
   const int64_t rows = static_cast<int64_t>(p->seqlen_q) * (p->heads_q / p->cache.heads_kv);
-  r.row_blocks = static_cast<int>((rows + 15) / 16);
-  r.rows_pad = r.row_blocks * 16;
-  const int64_t units = static_cast<int64_t>(p->batch) * p->cache.heads_kv * r.row_blocks;
-  // One wave of three CTAs on each of 148 SMs; at least two 16-key groups for each of a CTA's warps.
-  int64_t s = p->num_splits > 0 ? p->num_splits : 148 * 3 / (units > 0 ? units : 1);
-  const int64_t most = (p->max_seqlen_k + 127) / 128;
+  r.chunk = rows > 16;
+  const int per_block = r.chunk ? 256 : 16;
+  r.row_blocks = static_cast<int>((rows + per_block - 1) / per_block);
+  r.rows_pad = r.row_blocks * per_block;
+  int64_t units = static_cast<int64_t>(p->batch) * p->cache.heads_kv * r.row_blocks;
+  if (units < 1) units = 1;
+  // Few rows: one wave of three CTAs on each of 148 SMs, at least two 16-key groups for each of a
+  // CTA's warps. Many rows: one wave of one CTA an SM, at least four 128-key tiles each.
+  const int unit_keys = r.chunk ? 128 : 64;
+  int64_t s = p->num_splits > 0 ? p->num_splits : (r.chunk ? 148 : 148 * 3) / units;
+  const int64_t least = p->num_splits > 0 ? unit_keys : r.chunk ? 512 : 128;
+  const int64_t most = (p->max_seqlen_k + least - 1) / least;
   if (s > most) s = most;
   if (s > MAX_SPLITS) s = MAX_SPLITS;
   if (s < 1) s = 1;
   const int64_t per = (p->max_seqlen_k + s - 1) / s;
-  r.split_keys = static_cast<int>((per + 63) / 64 * 64);
-  if (r.split_keys < 64) r.split_keys = 64;
+  const int64_t keys = (per + unit_keys - 1) / unit_keys * unit_keys;
+  r.split_keys = static_cast<int>(keys < unit_keys ? unit_keys : keys > (1ll << 30) ? (1ll << 30) : keys);
   r.splits = static_cast<int>((static_cast<int64_t>(p->max_seqlen_k) + r.split_keys - 1) / r.split_keys);
   if (r.splits < 1) r.splits = 1;
   if (r.splits > 1) {
@@ -482,8 +491,11 @@ int check_core(const Fa2Kv8AttnParams* p) {
   // Row numbers and the grid stay in 31 bits.
   const int64_t rows = static_cast<int64_t>(p->seqlen_q) * (p->heads_q / p->cache.heads_kv);
   if (rows > (1ll << 30)) return FA2_ERR_SHAPE;
+  if (static_cast<int64_t>(p->batch) * p->cache.heads_kv > (1ll << 26)) return FA2_ERR_SHAPE;
   const Plan r = plan(p);
-  if (static_cast<int64_t>(p->batch) * p->cache.heads_kv * r.splits > (1ll << 30) / r.rows_pad * 4) return FA2_ERR_SHAPE;
+  if (static_cast<int64_t>(p->batch) * p->cache.heads_kv * r.splits > (1ll << 32) / (r.rows_pad > 0 ? r.rows_pad : 1)) {
+    return FA2_ERR_SHAPE;
+  }
   return FA2_OK;
 }
 
@@ -497,17 +509,27 @@ bool allow_smem(K kernel, int bytes, int dev, std::atomic<bool> (&done)[MAX_DEVI
 }
 
 template <int D, bool BF16>
-int launch(const AttnArgs& a, cudaStream_t s, int dev) {
-  static_assert(Dec<D>::SMEM <= 227 * 1024, "shared memory");
-  static std::atomic<bool> done[MAX_DEVICES];
-  auto kernel = decode_kernel<D, BF16>;
-  if (!allow_smem(kernel, Dec<D>::SMEM, dev, done)) return FA2_ERR_LAUNCH;
-  const int64_t ctas = static_cast<int64_t>(a.batch) * a.heads_kv * a.splits * a.row_blocks;
-  kernel<<<static_cast<unsigned>(ctas), DEC_WARPS * 32, Dec<D>::SMEM, s>>>(a);
-  int rc = launch_status();
+int launch(const AttnArgs& a, bool chunk, cudaStream_t s, int dev) {
+  static std::atomic<bool> done[2][MAX_DEVICES];
+  const unsigned ctas = static_cast<unsigned>(static_cast<int64_t>(a.batch) * a.heads_kv * a.splits * a.row_blocks);
+  if (chunk) {
+    auto kernel = chunk_kernel<D, BF16>;
+    if (!allow_smem(kernel, Ch<D>::SMEM, dev, done[1])) return FA2_ERR_LAUNCH;
+    kernel<<<ctas, CH_THREADS, Ch<D>::SMEM, s>>>(a);
+  } else {
+    auto kernel = decode_kernel<D, BF16>;
+    if (!allow_smem(kernel, Dec<D>::SMEM, dev, done[0])) return FA2_ERR_LAUNCH;
+    kernel<<<ctas, DEC_WARPS * 32, Dec<D>::SMEM, s>>>(a);
+  }
+  const int rc = launch_status();
   if (rc != FA2_OK || a.splits <= 1) return rc;
   const int64_t rows = static_cast<int64_t>(a.batch) * a.heads_kv * a.rows_pad;
-  merge_kernel<D, BF16, 16><<<static_cast<unsigned>((rows + 3) / 4), 128, 0, s>>>(a);
+  const unsigned blocks = static_cast<unsigned>((rows + 3) / 4);
+  if (chunk) {
+    merge_kernel<D, BF16, 256><<<blocks, 128, 0, s>>>(a);
+  } else {
+    merge_kernel<D, BF16, 16><<<blocks, 128, 0, s>>>(a);
+  }
   return launch_status();
 }
 
@@ -569,10 +591,10 @@ int fa2_kv8_attn_sm100(const Fa2Kv8AttnParams* p, void* stream) {
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf = p->dtype == FA2_DTYPE_BF16;
   switch (p->cache.head_dim) {
-    case 16: return bf ? launch<16, true>(a, s, dev) : launch<16, false>(a, s, dev);
-    case 32: return bf ? launch<32, true>(a, s, dev) : launch<32, false>(a, s, dev);
-    case 64: return bf ? launch<64, true>(a, s, dev) : launch<64, false>(a, s, dev);
-    default: return bf ? launch<128, true>(a, s, dev) : launch<128, false>(a, s, dev);
+    case 16: return bf ? launch<16, true>(a, r.chunk, s, dev) : launch<16, false>(a, r.chunk, s, dev);
+    case 32: return bf ? launch<32, true>(a, r.chunk, s, dev) : launch<32, false>(a, r.chunk, s, dev);
+    case 64: return bf ? launch<64, true>(a, r.chunk, s, dev) : launch<64, false>(a, r.chunk, s, dev);
+    default: return bf ? launch<128, true>(a, r.chunk, s, dev) : launch<128, false>(a, r.chunk, s, dev);
   }
 }
 
