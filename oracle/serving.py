@@ -52,15 +52,17 @@ def rows_of(codes, scales, block_table, b, n):
 
 def attention(q, cache, block_table, cache_seqlens, causal=True, sm_scale=None, causal_align="bottom_right",
               cu_seqlens_q=None):
-    """Returns (out, weight, spread): out as the operator defines it, weight = sum_j p_ij |v_j| / sum_j
-    p_ij (the same average of the magnitudes, for error bounds) and spread [.., H] the largest sum_d
-    |q_d k_d| * sm_scale of a row, all float64."""
+    """Returns (out, weight, spread, small): out as the operator defines it, weight = sum_j p_ij |v_j| /
+    sum_j p_ij (the same average of the magnitudes, for error bounds), spread [.., H] the largest sum_d
+    |q_d k_d| * sm_scale of a row and small [.., H] the largest max_d |q_d| * sum_d |k_d| * sm_scale, all
+    float64."""
     k, v, ks, vs = cache
     D = q.shape[-1]
     sm_scale = 1 / math.sqrt(D) if sm_scale is None else sm_scale
     group = q.shape[1] // k.shape[2]
     out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
-    weight, spread = torch.zeros_like(out), torch.zeros(q.shape[:-1], dtype=torch.float64, device=q.device)
+    weight = torch.zeros_like(out)
+    spread, small = (torch.zeros(q.shape[:-1], dtype=torch.float64, device=q.device) for _ in range(2))
     lens = [int(n) for n in cache_seqlens.tolist()]
     cu = [int(n) for n in cu_seqlens_q.tolist()] if cu_seqlens_q is not None else None
     for b, n in enumerate(lens):
@@ -83,8 +85,7 @@ def attention(q, cache, block_table, cache_seqlens, causal=True, sm_scale=None, 
             o = torch.stack([p[i, sees[i]] @ val[sees[i]] for i in range(n_q)]) if not torch.isfinite(val).all() else p @ val
             w = p @ val.abs()
             a = (qs[h].abs() @ keys[:, h // group].abs().T * sm_scale).masked_fill(~sees, 0).amax(-1)
-            if cu is not None:
-                out[rows, h], weight[rows, h], spread[rows, h] = o, w, a
-            else:
-                out[b, h], weight[b, h], spread[b, h] = o, w, a
-    return out, weight, spread
+            e = qs[h].abs().amax(-1) * keys[:, h // group].abs().sum(-1).amax() * sm_scale
+            at = (rows, h) if cu is not None else (b, h)
+            out[at], weight[at], spread[at], small[at] = o, w, a, e
+    return out, weight, spread, small

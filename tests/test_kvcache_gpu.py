@@ -196,7 +196,7 @@ def test_read_back(dtype, D, page_size):
 
 
 # ------------------------------------------------------------------------------------ attention
-def tolerance(q, weight, spread, out, n, v_top):
+def tolerance(q, weight, spread, small, out, n, v_top):
     """How far the kernel's output may be from the 64-bit one, element by element.
 
     A score x = sm_scale log2(e) sum q k is a fp32 sum of D exact products and two more roundings,
@@ -207,11 +207,12 @@ def tolerance(q, weight, spread, out, n, v_top):
     once: eps / 2, half a subnormal step at the bottom of fp16. What an element is off by is relative
     to weight = sum p |v| / sum p.
 
-    bf16 queries of many rows run on code * scale rounded to fp16 (half a step: 2^-11): a score is
-    off by 2^-11 spread more (log2(e) and ln(2) cancel), a value by 2^-11 of itself."""
+    Many rows: a query's values more than 2^10 below its row's largest are off by at most 2^-17 of
+    that one (e4m3 terms), which moves a score by 2^-17 small. Their bf16 queries also run on v * 2^k
+    rounded to fp16 (half a step: 2^-11 of the value)."""
     D = q.shape[-1]
     folded = 2.0 ** -11 if q.dtype == torch.bfloat16 else 0.0
-    dx = ((D + 8) * 2.0 ** -23 + folded) * spread[..., None] + 2.0 ** -22
+    dx = (D + 8) * 2.0 ** -23 * spread[..., None] + 2.0 ** -17 * small[..., None] + 2.0 ** -22
     rel = 2.0 ** -11 + folded + 2 * dx + 2 * n / 8 * 2.0 ** -23
     eps = torch.finfo(q.dtype).eps / 2
     return weight * rel * (1 + eps) + eps * out.abs() + n * 2.0 ** -31 * v_top + SUBNORMAL[q.dtype]
@@ -220,12 +221,12 @@ def tolerance(q, weight, spread, out, n, v_top):
 def check_attention(q, cache, bt, lens, **kw):
     got = attention_kvcache_fp8(q, cache, bt, lens, **kw)
     plain_kw = {k: kw[k] for k in ("causal", "sm_scale", "causal_align", "cu_seqlens_q") if k in kw}
-    out, weight, spread = serving.attention(q, cache, bt, lens, **plain_kw)
+    out, weight, spread, small = serving.attention(q, cache, bt, lens, **plain_kw)
     n = int(lens.max())
     v_top = max([serving.rows_of(cache[1], cache[3], bt, b, m).abs().max().item() for b, m in enumerate(lens.tolist()) if m] + [0.0])
     assert got.shape == q.shape and got.dtype == q.dtype
     end = q.shape[0] if q.dim() == 4 else int(kw["cu_seqlens_q"][-1])
-    err, tol = (got.double() - out).abs()[:end], tolerance(q, weight, spread, out, n, v_top)[:end]
+    err, tol = (got.double() - out).abs()[:end], tolerance(q, weight, spread, small, out, n, v_top)[:end]
     assert (err <= tol).all(), f"worst {(err / tol).max().item():.3f} of the tolerance, err {err.max().item():.3e}"
     return got
 
@@ -316,7 +317,7 @@ def test_attention_nonfinite_rows_reach_only_who_sees_them(N_q):
     out = attention_kvcache_fp8(q, cache, bt, sl)
     assert torch.isnan(out[:, :, N_q - 4:]).all()
     assert torch.isfinite(out[:, :, :N_q - 4]).all()
-    clean, _, _ = serving.attention(q[:, :, :N_q - 4], cache, bt, sl - 4)
+    clean, *_ = serving.attention(q[:, :, :N_q - 4], cache, bt, sl - 4)
     assert (out[:, :, :N_q - 4].double() - clean).abs().max() < 0.02  # (bounded tightly by the tests above)
     q[0, 2, 1, 5] = math.nan
     out = attention_kvcache_fp8(q, cache, bt, sl)
@@ -458,5 +459,5 @@ def test_two_graphs_and_a_side_stream(N_q):
         torch.cuda.synchronize()
         assert torch.equal(outs[0], eager)
         assert torch.equal(outs[1], attention_kvcache_fp8(qs[1], cache, bt, sl, num_splits=5))
-        ref, weight, spread = serving.attention(qs[1], cache, bt, sl)
-        assert ((outs[1].double() - ref).abs() <= tolerance(qs[1], weight, spread, ref, 2000, 8.0)).all()
+        ref, weight, spread, small = serving.attention(qs[1], cache, bt, sl)
+        assert ((outs[1].double() - ref).abs() <= tolerance(qs[1], weight, spread, small, ref, 2000, 8.0)).all()

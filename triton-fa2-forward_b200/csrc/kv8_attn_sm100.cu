@@ -514,8 +514,8 @@ int launch(const AttnArgs& a, bool chunk, cudaStream_t s, int dev) {
   const unsigned ctas = static_cast<unsigned>(static_cast<int64_t>(a.batch) * a.heads_kv * a.splits * a.row_blocks);
   if (chunk) {
     auto kernel = chunk_kernel<D, BF16>;
-    if (!allow_smem(kernel, Ch<D>::SMEM, dev, done[1])) return FA2_ERR_LAUNCH;
-    kernel<<<ctas, CH_THREADS, Ch<D>::SMEM, s>>>(a);
+    if (!allow_smem(kernel, Ch<D, BF16>::SMEM, dev, done[1])) return FA2_ERR_LAUNCH;
+    kernel<<<ctas, CH_THREADS, Ch<D, BF16>::SMEM, s>>>(a);
   } else {
     auto kernel = decode_kernel<D, BF16>;
     if (!allow_smem(kernel, Dec<D>::SMEM, dev, done[0])) return FA2_ERR_LAUNCH;

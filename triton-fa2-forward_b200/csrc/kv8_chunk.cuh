@@ -1,21 +1,30 @@
 // Attention over the 8-bit paged cache for many rows (chunks of prompts): tcgen05 products.
 //
 // Bound by the tensor cores (4 D operations a score) and, inside a step, by the exponentials
-// (16 a clock and SM) and shared memory. A CTA owns 256 rows (queries x heads of a group) as two
-// 128-row tiles that take turns: while one tile's scores go through the softmax, the tensor core
-// works on the other. With 128 rows or fewer both tiles hold the same rows and take every other
-// 128-key tile, merged at the end.
+// (16 a clock and SM), the issue slots and shared memory. A CTA owns 256 rows (queries x heads of a
+// group) as two 128-row tiles that take turns: while one tile's scores go through the softmax, the
+// tensor core works on the other. With 128 rows or fewer both tiles hold the same rows and take
+// every other 128-key tile, merged at the end.
+//
+// QK^T runs on the codes as they are stored: K is an e4m3 operand, and a row of Q, times the power
+// of two that brings its largest value into [128, 256), is the sum of two e4m3 operands for bf16
+// (8 significant bits: 4 and a sign's 4) or three for fp16 (11 bits). That is exact but for values
+// more than 2^10 below the row's largest, which are off by at most 2^-17 of it. 8-bit products run
+// at twice the rate of 16-bit ones, so the second operand costs nothing over converting K to fp16
+// (64 instructions less for each 16 values).
+//
+// PV runs on fp16: P' needs 11 bits. V is converted on its way into shared memory. Its row scales:
+// bf16 queries fold them into that conversion (code * s_j in fp16, one rounding of at most 2^-11, an
+// eighth of the output's half step); for fp16 queries, whose half step is 2^-11 itself, the codes
+// stay exact and each probability is multiplied by its key's scale in fp32. K's scales multiply the
+// scores.
 //
 // Warps 0-3 / 4-7: softmax of tile 0 / 1, one thread a row (scores and P' live in TMEM, P' feeds the
-// second product from there). Warps 8-10: bring the codes of 128-key tiles in from their pages and
-// convert them to fp16, swizzled as the tensor core reads them, through a ring of three 16-bit
-// tiles. Warp 11: issues the products.
-//
-// Where the row scales go. bf16 queries: into the conversion (code * s_j in fp16, one rounding of at
-// most 2^-11, an eighth of the output's half step), which leaves nothing to do for each score. fp16
-// queries, whose half step is 2^-11 itself: the codes stay exact and each score and probability is
-// multiplied by its key's scale in fp32.
+// second product from there). Warps 8-11: bring the tiles in from their pages: K by asynchronous
+// copies, two tiles ahead, V through registers. Warp 12: issues the products.
 #pragma once
+
+#include <type_traits>
 
 #include "kv8_attn.cuh"
 
@@ -26,64 +35,87 @@ using fa2::mbar_init;
 using fa2::mbar_wait;
 using fa2::mbar_wait_warp;
 using fa2::mma_commit;
-using fa2::mma_ss;
-using fa2::mma_ts;
 using fa2::smem_u32;
 using fa2::tc_fence_after;
 using fa2::tc_fence_before;
 
-constexpr int CH_THREADS = 384;
-constexpr int CH_CONV_WARP = 8, CH_CONV_THREADS = 96, CH_MMA_WARP = 11;
-constexpr int CH_SLOTS = 3;     // ring of converted tiles
-constexpr int CH_ENTRIES = 8;   // ring of the tiles' scales
-constexpr int CH_REGS = 168;    // a thread at launch; then CH_REGS_SM / CH_REGS_OTHER
-constexpr int CH_REGS_SM = 200, CH_REGS_OTHER = 104;
-static_assert(256 * CH_REGS_SM + 128 * CH_REGS_OTHER <= CH_THREADS * CH_REGS, "register split");
+constexpr int CH_THREADS = 512;
+constexpr int CH_CONV_WARP = 8, CH_CONV_THREADS = 128, CH_MMA_WARP = 12;
+constexpr int CH_KSLOTS = 3, CH_VSLOTS = 2;  // rings of K (codes) and V (fp16) tiles
+constexpr int CH_ENTRIES = 8;                // ring of the tiles' scales
+constexpr int CH_REGS = 128;                 // a thread at launch, then by warpgroup:
+constexpr int CH_REGS_SM = 176, CH_REGS_CONV = 88, CH_REGS_MMA = 72;
+static_assert(256 * CH_REGS_SM + 128 * CH_REGS_CONV + 128 * CH_REGS_MMA <= CH_THREADS * CH_REGS, "register split");
 constexpr long long CH_TIMEOUT = 2000000000ll;
 constexpr int FOLD_SHIFT = 6;   // folded scales: the largest lies in [2^6, 2^7), times 448 below 2^16
 
-template <int D>
+template <int D, bool BF16>
 struct Ch {
-  static constexpr int CHUNKS = D > 64 ? D / 64 : 1;  // 64-column pieces of a 16-bit tile
-  static constexpr int CHUNK = 128 * 128;             // bytes
-  static constexpr int TILE = CHUNKS * CHUNK;
-  static constexpr int OFF_Q = 0;
-  static constexpr int OFF_RING = 2 * TILE;
-  static constexpr int OFF_SC = OFF_RING + CH_SLOTS * TILE;     // [entry][2][128] words
-  static constexpr int OFF_HEAD = OFF_SC + CH_ENTRIES * 1024;   // [entry]{key scale of the tile, exponent of sv}
-  static constexpr int OFF_MAX = OFF_HEAD + CH_ENTRIES * 8;     // [2][3 warps][2]
-  static constexpr int OFF_BAR = OFF_MAX + 64;
+  static constexpr int TERMS = BF16 ? 2 : 3;          // e4m3 operands of Q
+  static constexpr int KSTEPS = D > 32 ? D / 32 : 1;  // 32-wide steps of QK^T (D = 16: zeros beyond)
+  static constexpr int CODES = 128 * 128;             // bytes of a tile of codes: 128-byte rows
+  static constexpr int CHUNKS = D > 64 ? D / 64 : 1;  // 64-column pieces of an fp16 tile
+  static constexpr int CHUNK = 128 * 128;
+  static constexpr int VTILE = CHUNKS * CHUNK;
+  static constexpr int OFF_Q = 0;  // [tile][term]
+  static constexpr int OFF_K = 2 * TERMS * CODES;
+  static constexpr int OFF_V = OFF_K + CH_KSLOTS * CODES;
+  static constexpr int OFF_SC = OFF_V + CH_VSLOTS * VTILE;      // [entry][2][128] words
+  static constexpr int OFF_HEAD = OFF_SC + CH_ENTRIES * 1024;   // [entry] exponent field of sv
+  static constexpr int OFF_MAX = OFF_HEAD + CH_ENTRIES * 4;     // [2][4 warps]
+  static constexpr int OFF_BAR = OFF_MAX + 32;
   static constexpr int OFF_TMEM = OFF_BAR + 256;
   static constexpr int SMEM = OFF_TMEM + 16 + 1024;             // and slack to align the base
-  // The merge of two tiles of the same rows: O of tile 1 in fp32 over the ring and what follows it.
-  static constexpr int MERGE = 128 * D * 4 + 2 * 128 * 4 + 512;
-  static_assert(OFF_RING + MERGE <= OFF_HEAD, "merge area");
+  // The merge of two tiles of the same rows: O of tile 1 in fp32 over the rings.
+  static constexpr int MERGE = 128 * D * 4 + 2 * 128 * 4;
+  static_assert(OFF_K + MERGE <= OFF_SC, "merge area");
   static_assert(SMEM <= 227 * 1024, "shared memory");
   static constexpr int TMEM_O = 256;
 };
 
-enum ChBar { CB_Q = 0, CB_S = 2, CB_P = 4, CB_PL = 6, CB_O = 8, CB_FULL = 10, CB_EMPTY = CB_FULL + CH_SLOTS,
-             CB_SC = CB_EMPTY + CH_SLOTS, CB_DONE = CB_SC + CH_ENTRIES, CB_COUNT };
+enum ChBar { CB_Q = 0, CB_S = 2, CB_P = 4, CB_PL = 6, CB_O = 8, CB_KF = 10, CB_KE = CB_KF + CH_KSLOTS,
+             CB_VF = CB_KE + CH_KSLOTS, CB_VE = CB_VF + CH_VSLOTS, CB_SC = CB_VE + CH_VSLOTS,
+             CB_DONE = CB_SC + CH_ENTRIES, CB_COUNT };
 static_assert(CB_COUNT * 8 <= 256, "barriers");
 
-// Order of the converted tiles, which is the order of the products: the first `ahead` K tiles, then
-// V_n, K_(n + ahead) in turn, then the V tiles that are left. i -> (is V, n).
-struct TileOrder {
-  int tiles, ahead;
-  __device__ void at(int i, bool& is_v, int& n) const {
-    if (i < ahead) {
-      is_v = false;
-      n = i;
-    } else if (i < 2 * tiles - ahead) {
-      const int k = i - ahead;
-      is_v = (k & 1) == 0;
-      n = (k >> 1) + (is_v ? 0 : ahead);
-    } else {
-      is_v = true;
-      n = i - tiles;
-    }
+// A shared-memory descriptor's upper word (128-byte swizzle, 8-row groups 1024 bytes apart), and the
+// lower one of a tile at `addr` with `lbo` bytes between 64-column pieces.
+constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) { return ((addr >> 4) & 0x3fffu) | ((lbo >> 4) << 16); }
+
+// The products take their operands as tile + compile-time offset and put the descriptor together in
+// place: kept in variables, the unrolled steps' descriptors cost the issuing thread 50 registers.
+// D[tmem] (+)= A[smem] * B[smem], both e4m3 (32 wide steps), fp32 sums.
+template <int A_OFF, int B_OFF>
+__device__ __forceinline__ void mma_e4m3(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b32 x, y;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "add.u32 x, %1, %5;\n\tadd.u32 y, %2, %6;\n\tmov.b64 da, {x, %7};\n\tmov.b64 db, {y, %7};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(add), "n"(A_OFF >> 4), "n"(B_OFF >> 4), "r"(DESC_HI)
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem], both fp16 (16 wide steps).
+template <int A_OFF, int B_OFF>
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b32 x, y;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "add.u32 x, %1, %5;\n\tadd.u32 y, %2, %6;\n\tmov.b64 db, {y, %7};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [x], db, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(add), "n"(A_OFF), "n"(B_OFF >> 4), "r"(DESC_HI)
+      : "memory");
+}
+template <int I, int N, typename F>
+__device__ __forceinline__ void steps(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    steps<I + 1, N>(static_cast<F&&>(f));
   }
-};
+}
+// Instruction descriptor of kind::f8f6f4: fp32 D, e4m3 A and B (type codes 0), both K-major.
+__host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N) {
+  return (1u << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
 
 __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   uint32_t r;
@@ -104,19 +136,19 @@ __device__ __forceinline__ uint32_t split_scale(float s) {
          (static_cast<uint32_t>(__half_as_ushort(__float2half_rn(rest))) << 16);
 }
 
-// The three converting warps meet; false where one of them gave up, in all of them alike.
+// The four loading warps meet; false where one of them gave up, in all of them alike.
 __device__ __forceinline__ bool conv_sync(bool ok) {
   uint32_t bad = ok ? 0u : 1u;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %0, 0;\n\t"
-      "bar.red.or.pred q, 1, 96, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      "bar.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
       : "+r"(bad)::"memory");
   return bad == 0;
 }
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) {
-  using C = Ch<D>;
+  using C = Ch<D, BF16>;
   constexpr bool FOLD = BF16;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t sraw = smem_u32(smem_raw);
@@ -150,9 +182,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
     return;
   }
   const bool dual = n_rows <= 128;
-  TileOrder order;
-  order.tiles = tiles;
-  order.ahead = dual && tiles > 1 ? 2 : 1;
+  const int ahead = dual && tiles > 1 ? 2 : 1;  // score tiles under way
   const long long timeout = a.timeout > 0 ? a.timeout : CH_TIMEOUT;
 
   if (threadIdx.x == 0) {
@@ -163,9 +193,13 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
       mbar_init(bar(CB_PL + t), 128);
       mbar_init(bar(CB_O + t), 1);
     }
-    for (int s = 0; s < CH_SLOTS; ++s) {
-      mbar_init(bar(CB_FULL + s), CH_CONV_THREADS);
-      mbar_init(bar(CB_EMPTY + s), 1);
+    for (int s = 0; s < CH_KSLOTS; ++s) {
+      mbar_init(bar(CB_KF + s), CH_CONV_THREADS);
+      mbar_init(bar(CB_KE + s), 1);
+    }
+    for (int s = 0; s < CH_VSLOTS; ++s) {
+      mbar_init(bar(CB_VF + s), CH_CONV_THREADS);
+      mbar_init(bar(CB_VE + s), 1);
     }
     for (int s = 0; s < CH_ENTRIES; ++s) mbar_init(bar(CB_SC + s), CH_CONV_THREADS);
     mbar_init(bar(CB_DONE), 1);
@@ -184,11 +218,10 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
   bool ok = true;
 
   if (warp >= CH_CONV_WARP && warp < CH_MMA_WARP) {
-    // -------------------------------------------------------------- codes -> fp16 tiles
-    fa2::reg_dealloc<CH_REGS_OTHER>();
+    // -------------------------------------------------------------- K codes, V codes -> fp16
+    fa2::reg_dealloc<CH_REGS_CONV>();
     const int tid = static_cast<int>(threadIdx.x) - CH_CONV_WARP * 32;
-    constexpr int PIECES = D / 16;                                     // 16-byte pieces of a row
-    constexpr int N_IT = (128 * PIECES + CH_CONV_THREADS - 1) / CH_CONV_THREADS;
+    constexpr int PIECES = D / 16;  // 16-byte pieces of a row
     const int* bt = a.bt + b * a.bt_stride;
     const int ps = a.c.page_size;
     const bool small = ps < 128;
@@ -196,252 +229,267 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
     // Pages of a tile: lane l holds page slot l's index (-1: no keys there, -2: refused).
     auto pages_of = [&](int n) -> int {
       const int key = k0 + n * 128 + lane * ps;
-      if (lane >= slots || key >= sq.len) return -1;
-      const int pg = __ldg(bt + page_of(a.c, small ? key : k0 + n * 128));
+      if (lane >= slots || key >= sq.len || n >= tiles) return -1;
+      const int pg = __ldg(bt + page_of(a.c, key));
       return pg >= 0 && pg < a.c.num_pages ? pg : -2;
     };
-    auto page_row = [&](int pg, int n, int r, int& row) -> int {
-      row = small ? r & (ps - 1) : (k0 + n * 128) % ps + r;
-      return __shfl_sync(0xffffffffu, pg, small ? r >> a.c.page_shift : 0);
-    };
-    uint4 w[N_IT];  // the next tile's codes, in flight
-    auto fetch_piece = [&](int it, int n, bool is_v, int pg) {
-      const int e = it * CH_CONV_THREADS + tid;
-      const int r = min(e / PIECES, 127), piece = e % PIECES;
-      int row;
-      const int page = page_row(pg, n, r, row);  // a shuffle: every lane
-      w[it] = make_uint4(0, 0, 0, 0);
-      if (e < 128 * PIECES && page >= 0 && k0 + n * 128 + r < sq.len) {
-        const uint8_t* base = is_v ? a.c.v + h * a.c.v_st[2] + page * a.c.v_st[0] + row * a.c.v_st[1]
-                                   : a.c.k + h * a.c.k_st[2] + page * a.c.k_st[0] + row * a.c.k_st[1];
-        w[it] = __ldg(reinterpret_cast<const uint4*>(base + piece * 16));
+    const uint8_t* kh = a.c.k + h * a.c.k_st[2];
+    const uint8_t* vh = a.c.v + h * a.c.v_st[2];
+
+    // K: thread tid copies piece tid % PIECES of the rows tid / PIECES + K_ROWS * it, to rows of 128
+    // bytes whose 16-byte parts are xor-ed with the row's number (128-byte swizzle).
+    constexpr int K_ROWS = CH_CONV_THREADS / PIECES, K_IT = PIECES;
+    const int k_row = tid / PIECES, k_piece = tid % PIECES;
+    auto copy_k = [&](int n, int pg) {
+      const uint32_t slot = sbase + C::OFF_K + (n % CH_KSLOTS) * C::CODES;
+      const int keys = sq.len - (k0 + n * 128);
+      const int page0 = __shfl_sync(0xffffffffu, pg, 0);
+      const uint8_t* p0 = kh + k_piece * 16;
+      if (!small) p0 += max(page0, 0) * a.c.k_st[0] + static_cast<int64_t>((k0 + n * 128) % ps + k_row) * a.c.k_st[1];
+#pragma unroll
+      for (int it = 0; it < K_IT; ++it) {
+        const int r = it * K_ROWS + k_row;
+        int page = page0;
+        const uint8_t* p = p0 + it * K_ROWS * a.c.k_st[1];
+        if (small) {
+          page = __shfl_sync(0xffffffffu, pg, r >> a.c.page_shift);
+          p = p0 + max(page, 0) * a.c.k_st[0] + (r & (ps - 1)) * a.c.k_st[1];
+        }
+        const bool in = r < keys && page >= 0;
+        cp_async16(slot + r * 128 + ((k_piece ^ (r & 7)) << 4), in ? p : kh, in);
       }
     };
-    float sc[2][2] = {};  // (key tid, key tid + 96) x (sk, sv) of the next K tile
-    auto fetch_scales = [&](int n, int pg) {
+
+    // V: thread tid has piece tid % PC of the rows tid / PC + V_ROWS * it, 64 columns at a time, so
+    // that eight neighbouring lanes write two rows and do not meet in a bank.
+    constexpr int PC = PIECES < 4 ? PIECES : 4;
+    constexpr int V_ROWS = CH_CONV_THREADS / PC, V_IT = 128 / V_ROWS * C::CHUNKS;
+    const int v_row = tid / PC, v_piece = tid % PC;
+    uint4 w[V_IT];  // the next tile's codes, in flight
+    auto fetch_v = [&](int n, int pg) {
+      const int keys = sq.len - (k0 + n * 128);
+      const int page0 = __shfl_sync(0xffffffffu, pg, 0);
+      const uint8_t* p0 = vh + v_piece * 16;
+      if (!small) {
+        p0 += max(page0, 0) * a.c.v_st[0] + static_cast<int64_t>((k0 + n * 128) % ps + v_row) * a.c.v_st[1];
+        if (page0 >= 0 && keys >= 128) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = min(tid + 96 * i, 127);
-        int row;
-        const int page = page_row(pg, n, r, row);
-        sc[i][0] = sc[i][1] = page == -2 ? __uint_as_float(0x7fc00000u) : 0.0f;
-        if (page >= 0 && k0 + n * 128 + r < sq.len) {
-          sc[i][0] = __ldg(a.c.ks + h * a.c.ks_st[2] + page * a.c.ks_st[0] + row * a.c.ks_st[1]);
-          sc[i][1] = __ldg(a.c.vs + h * a.c.vs_st[2] + page * a.c.vs_st[0] + row * a.c.vs_st[1]);
+          for (int it = 0; it < V_IT; ++it) {
+            w[it] = __ldg(reinterpret_cast<const uint4*>(p0 + (it % (128 / V_ROWS)) * V_ROWS * a.c.v_st[1] + it / (128 / V_ROWS) * 64));
+          }
+          return;
         }
-        // A value row that is not finite makes its key's score NaN instead (0 * NaN in the second
-        // product would reach the rows that do not see the key).
-        if (!(fabsf(sc[i][1]) < INFINITY)) {
-          sc[i][0] = __uint_as_float(0x7fc00000u);
-          sc[i][1] = 0.0f;
+      }
+#pragma unroll
+      for (int it = 0; it < V_IT; ++it) {
+        const int r = (it % (128 / V_ROWS)) * V_ROWS + v_row;
+        int page = page0;
+        const uint8_t* p = p0 + (it % (128 / V_ROWS)) * V_ROWS * a.c.v_st[1] + it / (128 / V_ROWS) * 64;
+        if (small) {
+          page = __shfl_sync(0xffffffffu, pg, r >> a.c.page_shift);
+          p = p0 + max(page, 0) * a.c.v_st[0] + (r & (ps - 1)) * a.c.v_st[1] + it / (128 / V_ROWS) * 64;
         }
-        if (page == -2 && tid + 96 * i < 128 && k0 + n * 128 + r < sq.len) report(a.err, FA2_ERR_PAGE);
+        w[it] = make_uint4(0, 0, 0, 0);
+        if (r < keys && page >= 0) w[it] = __ldg(reinterpret_cast<const uint4*>(p));
+      }
+    };
+    auto convert_v = [&](int n) {
+      uint8_t* dst = smem + C::OFF_V + (n % CH_VSLOTS) * C::VTILE + v_row * 128;
+      const uint32_t part = (static_cast<uint32_t>(v_piece) * 2) ^ static_cast<uint32_t>(v_row & 7);
+      const uint32_t* sc = reinterpret_cast<const uint32_t*>(smem + C::OFF_SC) + (n % CH_ENTRIES) * 256 + 128 + v_row;
+      uint32_t ws[V_IT];
+#pragma unroll
+      for (int it = 0; it < V_IT; ++it) ws[it] = FOLD ? sc[(it % (128 / V_ROWS)) * V_ROWS] : 0u;
+#pragma unroll
+      for (int it = 0; it < V_IT; ++it) {
+        const uint32_t c[4] = {w[it].x, w[it].y, w[it].z, w[it].w};
+        uint32_t o[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          o[2 * i] = f16x2_of_e4m3x2(static_cast<uint16_t>(c[i]));
+          o[2 * i + 1] = f16x2_of_e4m3x2(static_cast<uint16_t>(c[i] >> 16));
+        }
+        if constexpr (FOLD) {
+          const uint32_t hi = __byte_perm(ws[it], ws[it], 0x1010), lo = __byte_perm(ws[it], ws[it], 0x3232);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i] = hfma2(o[i], hi, hmul2(o[i], lo));
+        }
+        uint8_t* row = dst + (it % (128 / V_ROWS)) * V_ROWS * 128 + it / (128 / V_ROWS) * C::CHUNK;
+        *reinterpret_cast<uint4*>(row + (part << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+        *reinterpret_cast<uint4*>(row + ((part ^ 1u) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+      }
+    };
+    static_assert(V_ROWS % 8 == 0, "a thread's rows have the same swizzle");
+
+    float sk = 0.0f, sv = 0.0f;  // of key tid of the next tile
+    auto fetch_scales = [&](int n, int pg) {
+      const int page = __shfl_sync(0xffffffffu, pg, small ? tid >> a.c.page_shift : 0);
+      const int row = small ? tid & (ps - 1) : (k0 + n * 128) % ps + tid;
+      const bool in = k0 + n * 128 + tid < sq.len;
+      sk = sv = 0.0f;
+      if (page >= 0 && in) {
+        sk = __ldg(a.c.ks + h * a.c.ks_st[2] + page * a.c.ks_st[0] + row * a.c.ks_st[1]);
+        sv = __ldg(a.c.vs + h * a.c.vs_st[2] + page * a.c.vs_st[0] + row * a.c.vs_st[1]);
+      } else if (page == -2 && in) {  // queries that see a key of a refused page get NaN
+        sv = __uint_as_float(0x7fc00000u);
+        report(a.err, FA2_ERR_PAGE);
       }
     };
     int eb = EB_MIN;  // exponent field of the largest finite sv so far
-    // Scales of tile n, from sc: into its entry, with the tile's exponents.
+    // Scales of tile n into its entry, and the exponent that they are relative to.
     auto store_scales = [&](int n) {
-      uint32_t top[2] = {0, 0};
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (tid + 96 * i < 128) {
-#pragma unroll
-          for (int z = 0; z < 2; ++z) {
-            const uint32_t v = __float_as_uint(sc[i][z]) & 0x7fffffffu;
-            if (v < 0x7f800000u) top[z] = max(top[z], v);
-          }
-        }
+      // A value row that is not finite makes its key's score NaN instead (0 * NaN in the second
+      // product would reach the rows that do not see the key).
+      if (!(fabsf(sv) < INFINITY)) {
+        sk = __uint_as_float(0x7fc00000u);
+        sv = 0.0f;
       }
-      top[0] = __reduce_max_sync(0xffffffffu, top[0]);
-      top[1] = __reduce_max_sync(0xffffffffu, top[1]);
-      uint32_t* wm = reinterpret_cast<uint32_t*>(smem + C::OFF_MAX) + (n & 1) * 6;
-      if (lane < 2) wm[(warp - CH_CONV_WARP) * 2 + lane] = top[lane];
+      const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(sv) & 0x7fffffffu);
+      uint32_t* wm = reinterpret_cast<uint32_t*>(smem + C::OFF_MAX) + (n & 1) * 4;
+      if (lane == 0) wm[warp - CH_CONV_WARP] = top;
       conv_sync(true);
-      const int ek = max(EB_MIN, static_cast<int>(max(wm[0], max(wm[2], wm[4])) >> 23));
-      eb = max(eb, static_cast<int>(max(wm[1], max(wm[3], wm[5])) >> 23));
+      eb = max(eb, static_cast<int>(max(max(wm[0], wm[1]), max(wm[2], wm[3])) >> 23));
       const int en = n % CH_ENTRIES;
-      uint32_t* dst = reinterpret_cast<uint32_t*>(smem + C::OFF_SC) + en * 256;
-      const float fk = __uint_as_float(static_cast<uint32_t>(254 + FOLD_SHIFT - ek) << 23);
       const float fv = __uint_as_float(static_cast<uint32_t>(254 + FOLD_SHIFT - eb) << 23);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = tid + 96 * i;
-        if (r < 128) {
-          dst[r] = FOLD ? split_scale(sc[i][0] * fk) : __float_as_uint(sc[i][0]);
-          dst[128 + r] = FOLD ? split_scale(sc[i][1] * fv) : __float_as_uint(sc[i][1] * fv);
-        }
-      }
-      if (tid == 0) {
-        uint32_t* head = reinterpret_cast<uint32_t*>(smem + C::OFF_HEAD) + en * 2;
-        // 2^(ek - 127 - FOLD_SHIFT): what a folded score is to be multiplied by.
-        head[0] = FOLD ? (static_cast<uint32_t>(max(1, ek - FOLD_SHIFT)) << 23) : 0x3f800000u;
-        head[1] = static_cast<uint32_t>(eb);
-      }
+      uint32_t* dst = reinterpret_cast<uint32_t*>(smem + C::OFF_SC) + en * 256 + tid;
+      dst[0] = __float_as_uint(sk);
+      dst[128] = FOLD ? split_scale(sv * fv) : __float_as_uint(sv * fv);
+      if (tid == 0) reinterpret_cast<int*>(smem + C::OFF_HEAD)[en] = eb;
       mbar_arrive(bar(CB_SC + en));
       if (FOLD) conv_sync(true);  // the conversion reads the scales of the others' keys
     };
-    auto store_piece = [&](int it, int n, bool is_v, uint32_t dst) {
-      const int e = it * CH_CONV_THREADS + tid;
-      if (128 * PIECES % CH_CONV_THREADS != 0 && e >= 128 * PIECES) return;
-      const int r = e / PIECES, piece = e % PIECES;
-      const uint32_t c[4] = {w[it].x, w[it].y, w[it].z, w[it].w};
-      uint32_t o[8];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        o[2 * i] = f16x2_of_e4m3x2(static_cast<uint16_t>(c[i]));
-        o[2 * i + 1] = f16x2_of_e4m3x2(static_cast<uint16_t>(c[i] >> 16));
-      }
-      if constexpr (FOLD) {
-        const uint32_t s = reinterpret_cast<const uint32_t*>(smem + C::OFF_SC)[(n % CH_ENTRIES) * 256 + (is_v ? 128 : 0) + r];
-        const uint32_t hi = __byte_perm(s, s, 0x1010), lo = __byte_perm(s, s, 0x3232);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = hfma2(o[i], hi, hmul2(o[i], lo));
-      }
-      // 64 columns a 128-byte row, 16-byte parts xor-ed with the row's number (128-byte swizzle).
-      // The upper half of a row stores its parts in the other order: no two lanes meet in a bank.
-      const uint32_t row = dst + (piece >> 2) * C::CHUNK + r * 128;
-      const uint32_t flip = D > 64 ? static_cast<uint32_t>(piece >> 2) : 0u;
-      const uint32_t part = (static_cast<uint32_t>(piece & 3) * 2) ^ static_cast<uint32_t>(r & 7);
-      const bool f = flip != 0;
-      fa2::st_shared_v4(row + ((part ^ flip) << 4), f ? o[4] : o[0], f ? o[5] : o[1], f ? o[6] : o[2], f ? o[7] : o[3]);
-      fa2::st_shared_v4(row + ((part ^ flip ^ 1u) << 4), f ? o[0] : o[4], f ? o[1] : o[5], f ? o[2] : o[6], f ? o[3] : o[7]);
-    };
 
-    // Tile i is converted from registers while tile i + 1 is fetched into them, piece by piece; the
-    // page numbers of tile i + 2 are on their way.
-    const int total = 2 * tiles;
-    bool cur_v = false, next_v, then_v = false;
-    int cur_n = 0, next_n, then_n = 0, pg_next, pg_then = 0;
-    {
-      const int pg = pages_of(0);
-#pragma unroll
-      for (int it = 0; it < N_IT; ++it) fetch_piece(it, 0, false, pg);
-      fetch_scales(0, pg);
-    }
-    order.at(1, next_v, next_n);
-    pg_next = pages_of(next_n);
-    for (int i = 0; i < total; ++i) {
-      if (i + 2 < total) {
-        order.at(i + 2, then_v, then_n);
-        pg_then = pages_of(then_n);
+    if constexpr (D < 32) {  // the second half of the only 32-wide step
+      for (int i = tid; i < CH_KSLOTS * 128 * 8; i += CH_CONV_THREADS) {
+        *reinterpret_cast<uint4*>(smem + C::OFF_K + i * 16) = make_uint4(0, 0, 0, 0);
       }
-      const int slot = i % CH_SLOTS;
-      const uint32_t ph = static_cast<uint32_t>(i / CH_SLOTS) & 1u;
-      ok = conv_sync(mbar_wait_warp(bar(CB_EMPTY + slot), ph ^ 1u, timeout, a.err));
+      conv_sync(true);
+    }
+    // Step n: K_n has landed; K_(n + 2) is asked for; V_n is converted from registers and V_(n + 1)
+    // fetched into them. The page numbers of tile n + 3 are on their way.
+    int pg0 = pages_of(0), pg1 = pages_of(1), pg2 = pages_of(2);
+    copy_k(0, pg0);
+    cp_async_commit();
+    if (tiles > 1) copy_k(1, pg1);
+    cp_async_commit();
+    fetch_v(0, pg0);
+    fetch_scales(0, pg0);
+    for (int n = 0; n < tiles; ++n) {
+      const int pg3 = pages_of(n + 3);
+      bool go = true;
+      if (n + 2 < tiles) {
+        const int s = (n + 2) % CH_KSLOTS;
+        go = mbar_wait_warp(bar(CB_KE + s), (static_cast<uint32_t>((n + 2) / CH_KSLOTS) & 1u) ^ 1u, timeout, a.err);
+        if (go) copy_k(n + 2, pg2);
+      }
+      cp_async_commit();
+      cp_async_wait<2>();
+      fa2::fence_proxy_async_smem();
+      mbar_arrive(bar(CB_KF + n % CH_KSLOTS));
+      go = go && mbar_wait_warp(bar(CB_VE + n % CH_VSLOTS), (static_cast<uint32_t>(n / CH_VSLOTS) & 1u) ^ 1u, timeout, a.err);
+      ok = conv_sync(go);
       if (!ok) break;
-      if (!cur_v) store_scales(cur_n);
-      const uint32_t dst = sbase + C::OFF_RING + slot * C::TILE;
-      if (i + 1 < total) {
-#pragma unroll
-        for (int it = 0; it < N_IT; ++it) {
-          store_piece(it, cur_n, cur_v, dst);
-          fetch_piece(it, next_n, next_v, pg_next);
-        }
-        if (!next_v) fetch_scales(next_n, pg_next);
-      } else {
-#pragma unroll
-        for (int it = 0; it < N_IT; ++it) store_piece(it, cur_n, cur_v, dst);
+      store_scales(n);
+      convert_v(n);
+      if (n + 1 < tiles) {
+        fetch_v(n + 1, pg1);
+        fetch_scales(n + 1, pg1);
       }
       fa2::fence_proxy_async_smem();
-      mbar_arrive(bar(CB_FULL + slot));
-      cur_v = next_v;
-      cur_n = next_n;
-      next_v = then_v;
-      next_n = then_n;
-      pg_next = pg_then;
+      mbar_arrive(bar(CB_VF + n % CH_VSLOTS));
+      pg1 = pg2;
+      pg2 = pg3;
     }
+    cp_async_wait<0>();
   } else if (warp == CH_MMA_WARP) {
     // -------------------------------------------------------------- products
-    fa2::reg_dealloc<CH_REGS_OTHER>();
+    fa2::reg_dealloc<CH_REGS_MMA>();
     if (lane == 0) {
-      constexpr uint32_t idesc_qk = fa2::idesc_f16(false, 128, 128, false);
+      constexpr uint32_t idesc_qk = idesc_e4m3(128, 128);
       constexpr uint32_t idesc_pv = fa2::idesc_f16(false, 128, D, true);
-      const uint64_t dq = fa2::sdesc_sw128(sbase + C::OFF_Q, 16, 1024);
-      const uint64_t dk = fa2::sdesc_sw128(sbase + C::OFF_RING, 16, 1024);
-      const uint64_t dv = fa2::sdesc_sw128(sbase + C::OFF_RING, C::CHUNK, 1024);
+      const uint32_t dq = desc_lo(sbase + C::OFF_Q, 16), dk = desc_lo(sbase + C::OFF_K, 16);
+      const uint32_t dv = desc_lo(sbase + C::OFF_V, C::CHUNK);
       auto wait = [&](int i, uint32_t parity) -> bool { return mbar_wait(bar(i), parity, timeout, a.err); };
-      auto qk = [&](int t, int slot) {
-        const uint64_t qd = dq + static_cast<uint64_t>(((dual ? 0 : t) * C::TILE) >> 4);
-        const uint64_t kd = dk + static_cast<uint64_t>((slot * C::TILE) >> 4);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint64_t off = static_cast<uint64_t>(((kk >> 2) * C::CHUNK + (kk & 3) * 32) >> 4);
-          mma_ss(tmem + t * 128, qd + off, kd + off, idesc_qk, kk > 0 ? 1u : 0u);
-        }
+      auto qk = [&](int t, int n) {
+        const uint32_t qd = dq + static_cast<uint32_t>(((dual ? 0 : t) * C::TERMS * C::CODES) >> 4);
+        const uint32_t kd = dk + static_cast<uint32_t>(((n % CH_KSLOTS) * C::CODES) >> 4);
+        steps<0, C::TERMS * C::KSTEPS>([&](auto i) {
+          constexpr int term = decltype(i)::value / C::KSTEPS, kk = decltype(i)::value % C::KSTEPS;
+          mma_e4m3<term * C::CODES + kk * 32, kk * 32>(tmem + t * 128, qd, kd, idesc_qk, term + kk > 0 ? 1u : 0u);
+        });
         mma_commit(bar(CB_S + t));
       };
       // P' of tile t comes in two parts: 96 keys, then 32.
-      auto pv = [&](int t, int slot, bool acc, uint32_t parity) -> bool {
-        const uint64_t vd = dv + static_cast<uint64_t>((slot * C::TILE) >> 4);
+      auto pv = [&](int t, int n, bool acc, uint32_t parity) -> bool {
+        const uint32_t vd = dv + static_cast<uint32_t>(((n % CH_VSLOTS) * C::VTILE) >> 4);
+        const uint32_t td = tmem + C::TMEM_O + t * D, tp = tmem + t * 128 + 64;
         if (!wait(CB_P + t, parity)) return false;
         tc_fence_after();
-#pragma unroll
-        for (int kk = 0; kk < 6; ++kk) {
-          mma_ts(tmem + C::TMEM_O + t * D, tmem + t * 128 + 64 + kk * 8, vd + static_cast<uint64_t>((kk * 16 * 128) >> 4),
-                 idesc_pv, (acc || kk > 0) ? 1u : 0u);
-        }
+        steps<0, 6>([&](auto kk) {
+          mma_f16_ts<decltype(kk)::value * 8, decltype(kk)::value * 16 * 128>(td, tp, vd, idesc_pv, (acc || decltype(kk)::value > 0) ? 1u : 0u);
+        });
         if (!wait(CB_PL + t, parity)) return false;
         tc_fence_after();
-#pragma unroll
-        for (int kk = 6; kk < 8; ++kk) {
-          mma_ts(tmem + C::TMEM_O + t * D, tmem + t * 128 + 64 + kk * 8, vd + static_cast<uint64_t>((kk * 16 * 128) >> 4),
-                 idesc_pv, 1u);
-        }
+        mma_f16_ts<6 * 8, 6 * 16 * 128>(td, tp, vd, idesc_pv, 1u);
+        mma_f16_ts<7 * 8, 7 * 16 * 128>(td, tp, vd, idesc_pv, 1u);
         return true;
       };
-      int at = 0;  // place in the tile order
-      auto take = [&](int i) -> bool {
-        if (!wait(CB_FULL + i % CH_SLOTS, static_cast<uint32_t>(i / CH_SLOTS) & 1u)) return false;
+      auto take_k = [&](int n) -> bool {
+        if (!wait(CB_KF + n % CH_KSLOTS, static_cast<uint32_t>(n / CH_KSLOTS) & 1u)) return false;
         tc_fence_after();
         return true;
       };
-      auto drop = [&](int i) { mma_commit(bar(CB_EMPTY + i % CH_SLOTS)); };
+      auto take_v = [&](int n) -> bool {
+        if (!wait(CB_VF + n % CH_VSLOTS, static_cast<uint32_t>(n / CH_VSLOTS) & 1u)) return false;
+        tc_fence_after();
+        return true;
+      };
+      auto drop_k = [&](int n) { mma_commit(bar(CB_KE + n % CH_KSLOTS)); };
+      auto drop_v = [&](int n) { mma_commit(bar(CB_VE + n % CH_VSLOTS)); };
       ok = wait(CB_Q + 0, 0) && (dual || wait(CB_Q + 1, 0));
       if (ok && dual) {
-        for (int t = 0; ok && t < order.ahead; ++t) {
-          ok = take(at);
+        for (int n = 0; ok && n < ahead; ++n) {
+          ok = take_k(n);
           if (ok) {
-            qk(t, at % CH_SLOTS);
-            drop(at++);
+            qk(n & 1, n);
+            drop_k(n);
           }
         }
         for (int n = 0; ok && n < tiles; ++n) {
           const int t = n & 1;
-          ok = take(at) && pv(t, at % CH_SLOTS, n > 1, static_cast<uint32_t>(n >> 1) & 1u);
+          ok = take_v(n) && pv(t, n, n > 1, static_cast<uint32_t>(n >> 1) & 1u);
           if (!ok) break;
           if (n + 2 >= tiles) mma_commit(bar(CB_O + t));
-          drop(at++);
-          if (n + order.ahead < tiles) {
-            ok = take(at);
+          drop_v(n);
+          if (n + ahead < tiles) {
+            ok = take_k(n + ahead);
             if (!ok) break;
-            qk((n + order.ahead) & 1, at % CH_SLOTS);
-            drop(at++);
+            qk((n + ahead) & 1, n + ahead);
+            drop_k(n + ahead);
           }
         }
       } else if (ok) {
-        ok = take(at);
+        ok = take_k(0);
         if (ok) {
           qk(0, 0);
           qk(1, 0);
-          drop(at++);
+          drop_k(0);
         }
         for (int n = 0; ok && n < tiles; ++n) {
           const bool more = n + 1 < tiles;
           const uint32_t parity = static_cast<uint32_t>(n) & 1u;
-          const int iv = at, ik = at + 1;
           for (int t = 0; t < 2 && ok; ++t) {
-            ok = (t > 0 || take(iv)) && pv(t, iv % CH_SLOTS, n > 0, parity);
+            ok = (t > 0 || take_v(n)) && pv(t, n, n > 0, parity);
             if (!ok) break;
             if (!more) mma_commit(bar(CB_O + t));
-            if (t == 1) drop(iv);
+            if (t == 1) drop_v(n);
             if (more) {
-              ok = t > 0 || take(ik);
+              ok = t > 0 || take_k(n + 1);
               if (!ok) break;
-              qk(t, ik % CH_SLOTS);
-              if (t == 1) drop(ik);
+              qk(t, n + 1);
+              if (t == 1) drop_k(n + 1);
             }
           }
-          at += 2;
         }
       }
       // Every product has retired before TMEM is given back.
@@ -449,6 +497,8 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
       if (!mbar_wait(bar(CB_DONE), 0, CH_TIMEOUT, nullptr)) ok = false;
     }
     __syncwarp();
+  } else if (warp > CH_MMA_WARP) {
+    fa2::reg_dealloc<CH_REGS_MMA>();
   } else {
     // -------------------------------------------------------------- softmax: one thread a row
     fa2::reg_alloc<CH_REGS_SM>();
@@ -459,46 +509,15 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
     const uint32_t lane_addr = static_cast<uint32_t>(q * 32) << 16;
     const uint32_t tS = tmem + t * 128 + lane_addr, tP = tS + 64, tO = tmem + C::TMEM_O + t * D + lane_addr;
 
-    // Q: this row in fp16, times the power of two that brings its largest value below 2^15.
-    float row_sc = a.qk_scale;
-    if (!dual || t == 0) {
-      uint32_t w[D / 2];
+    // Q: this row as e4m3 terms, times the power of two that brings its largest value into [128, 256).
+    // Each term is the rounding of what the terms before leave (an exact difference in fp32).
+    float row_sc;
+    {
       uint32_t top = 0;
-      const uint16_t* src = q_row(a, sq, b, h, have ? row : row0);
+      const uint4* src = reinterpret_cast<const uint4*>(q_row(a, sq, b, h, have ? row : row0));
 #pragma unroll
       for (int i = 0; i < D / 8; ++i) {
-        const uint4 v = have ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
-        w[4 * i] = v.x;
-        w[4 * i + 1] = v.y;
-        w[4 * i + 2] = v.z;
-        w[4 * i + 3] = v.w;
-      }
-#pragma unroll
-      for (int i = 0; i < D / 2; ++i) {
-        const float2 v = float2_of_x2<BF16>(w[i]);
-        top = max(top, max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu));
-      }
-      const int e = row_exponent(top);
-      const float f = pow2f(14 - e);
-      row_sc = a.qk_scale * pow2f(max(-126, e - 14));
-      const uint32_t dst = sbase + C::OFF_Q + t * C::TILE + r * 128;
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        uint32_t o[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 v = float2_of_x2<BF16>(w[4 * i + j]);
-          o[j] = x2_of_floats<false>(v.x * f, v.y * f);
-        }
-        fa2::st_shared_v4(dst + (i >> 3) * C::CHUNK + (((i & 7) ^ (r & 7)) << 4), o[0], o[1], o[2], o[3]);
-      }
-      fa2::fence_proxy_async_smem();
-      mbar_arrive(bar(CB_Q + t));
-    } else {  // the same rows as tile 0's: only their scale
-      uint32_t top = 0;
-      const uint16_t* src = q_row(a, sq, b, h, have ? row : row0);
-      for (int i = 0; i < D / 8; ++i) {
-        const uint4 v = have ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
+        const uint4 v = have ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -506,7 +525,45 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
           top = max(top, max(__float_as_uint(f2.x) & 0x7fffffffu, __float_as_uint(f2.y) & 0x7fffffffu));
         }
       }
-      row_sc = a.qk_scale * pow2f(max(-126, row_exponent(top) - 14));
+      const int e = row_exponent(top);
+      const float f = top < 0x7f800000u ? pow2f(7 - e) : __uint_as_float(0x7fc00000u);  // NaN, infinity: a NaN row
+      row_sc = a.qk_scale * pow2f(max(-126, e - 7));
+      if (!dual || t == 0) {
+        const uint32_t dst = sbase + C::OFF_Q + t * C::TERMS * C::CODES + r * 128;
+#pragma unroll
+        for (int i = 0; i < (D + 15) / 16; ++i) {
+          float x[16];
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            const uint4 v = have ? __ldg(src + 2 * i + z) : make_uint4(0, 0, 0, 0);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 f2 = float2_of_x2<BF16>(w[j]);
+              x[8 * z + 2 * j] = f2.x * f;
+              x[8 * z + 2 * j + 1] = f2.y * f;
+            }
+          }
+#pragma unroll
+          for (int term = 0; term < C::TERMS; ++term) {
+            uint32_t o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint16_t lo = e4m3x2(x[4 * j], x[4 * j + 1]), hi = e4m3x2(x[4 * j + 2], x[4 * j + 3]);
+              const float2 y0 = float2_of_f16x2(f16x2_of_e4m3x2(lo)), y1 = float2_of_f16x2(f16x2_of_e4m3x2(hi));
+              x[4 * j] -= y0.x;
+              x[4 * j + 1] -= y0.y;
+              x[4 * j + 2] -= y1.x;
+              x[4 * j + 3] -= y1.y;
+              o[j] = static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
+            }
+            fa2::st_shared_v4(dst + term * C::CODES + ((i ^ (r & 7)) << 4), o[0], o[1], o[2], o[3]);
+            if constexpr (D < 32) fa2::st_shared_v4(dst + term * C::CODES + ((1 ^ (r & 7)) << 4), 0, 0, 0, 0);
+          }
+        }
+        fa2::fence_proxy_async_smem();
+        mbar_arrive(bar(CB_Q + t));
+      }
     }
     const int lim_row = have ? last_key(a, sq, row / a.group) : -1;  // last visible key
     const int tile_row0 = row0 + (dual ? 0 : t * 128);
@@ -525,32 +582,33 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
         break;
       }
       tc_fence_after();
-      const uint32_t head_addr = sbase + C::OFF_HEAD + en * 8;
       const uint32_t sc_addr = sbase + C::OFF_SC + en * 1024;
-      float k_sc;
       int eb_new;
-      asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=f"(k_sc), "=r"(eb_new) : "r"(head_addr));
-      const float sc = row_sc * k_sc;
+      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(eb_new) : "r"(sbase + C::OFF_HEAD + en * 4));
       const int col0 = k0 + n * 128;
+      const float sc = row_sc;
       const bool masked = col0 + 127 > lim_all;
       const int lim = lim_row - col0;
 
       uint32_t s[4][32];
-      fa2::tmem_ld128(tS, s[0], s[1], s[2], s[3]);
+      fa2::tmem_ld64(tS, s[0], s[1]);
+      fa2::tmem_ld64(tS + 64, s[2], s[3]);
       fa2::tmem_wait_ld();
 #pragma unroll
       for (int c = 0; c < 4; ++c) fa2::reg_fence32(s[c]);
-      if constexpr (!FOLD) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 4; ++c) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            float k[4];
-            asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];"
-                         : "=f"(k[0]), "=f"(k[1]), "=f"(k[2]), "=f"(k[3]) : "r"(sc_addr + (c * 32 + i) * 4));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[c][i + j] = __float_as_uint(__uint_as_float(s[c][i + j]) * k[j]);
-          }
+        for (int i = 0; i < 32; i += 4) {
+          uint64_t k0, k1;
+          asm volatile("ld.shared.v2.b64 {%0,%1}, [%2];" : "=l"(k0), "=l"(k1) : "r"(sc_addr + (c * 32 + i) * 4));
+          float u0, u1, u2, u3;
+          fa2::f2_unpack(fa2::f2_mul(fa2::f2_pack(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1])), k0), u0, u1);
+          fa2::f2_unpack(fa2::f2_mul(fa2::f2_pack(__uint_as_float(s[c][i + 2]), __uint_as_float(s[c][i + 3])), k1), u2, u3);
+          s[c][i] = __float_as_uint(u0);
+          s[c][i + 1] = __float_as_uint(u1);
+          s[c][i + 2] = __float_as_uint(u2);
+          s[c][i + 3] = __float_as_uint(u3);
         }
       }
       if (masked) {
@@ -647,7 +705,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
     tc_fence_after();
     const int ex = eb - 127 - FOLD_SHIFT;
     const float u0 = pow2f(ex / 2), u1 = pow2f(ex - ex / 2);
-    float* area = reinterpret_cast<float*>(smem + C::OFF_RING);  // [D / 4][128] float4
+    float* area = reinterpret_cast<float*>(smem + C::OFF_K);  // [D / 4][128] float4
     float* area_m = area + 128 * D;
     float* area_l = area_m + 128;
     if (dual) {
