@@ -1,13 +1,13 @@
 // Attention over the 8-bit paged cache: what its kernels share.
 //
-// With codes c and row scales s, and q scaled by a power of two f_i into fp16's range (exact):
+// With codes c and row scales s, and q scaled by a power of two f_i:
 //     x_ij = sm_scale * log2(e) / f_i * (sum_d q'_id ck_jd) * sk_j      p_ij = 2^(x_ij - m_i)
 //     o_i  = sum_j (p_ij sv_j) cv_j / sum_j p_ij
-// e4m3 codes are exact in fp16, so both products run on fp16 operands with fp32 sums whatever the
-// query's type, and the scales stay in fp32: sk_j multiplies the score's column, sv_j the
-// probability's. The only rounding to 16 bits inside is that of P' = p_ij sv_j 2^(6 - e) with e the
-// largest exponent of the sv seen so far (relative error 2^-11, below half a step of the output):
-// P' < 2^15 fits fp16, and the range down to 2^-24 reaches 2^-30 below the row's largest p.
+// The first product runs on fp16 operands for few rows (q' below 2^15, exact) and on e4m3 operands
+// for many (see there). The second runs on fp16: e4m3 codes are exact in it, and P' = p_ij sv_j
+// 2^(6 - e), with e the largest exponent of the sv seen so far, is rounded to it (relative error
+// 2^-11, below half a step of the output; P' < 2^15, and its range reaches 2^-30 below the row's
+// largest p). Sums, statistics and scales are fp32.
 #pragma once
 
 #include "kv8_common.cuh"
@@ -102,6 +102,9 @@ __device__ __forceinline__ int row_exponent(uint32_t top_bits) {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
   const int n = valid ? 16 : 0;  // 0: zeros are written, nothing is read
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async16_full(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool valid) {
   const int n = valid ? 4 : 0;

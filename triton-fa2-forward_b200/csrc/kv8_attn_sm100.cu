@@ -10,40 +10,55 @@ namespace {
 using namespace fa2kv;
 
 // ------------------------------------------------------------------ few rows (decode)
-// At most 16 rows (queries x heads of a group) a CTA. Bound by the bytes of the cache: 2 (D + 4) a
-// key. So the tensor work runs on warp-wide 16 x 8 x 16 products, which take the codes straight
-// from registers: every warp streams its own 16-key groups through its own ring of asynchronous
-// copies (no barrier between warps), converts them in registers and keeps its own running max, sum
-// and output; the four warps are merged once at the end. A 128-row tile would be 1/8 full at most
-// and its conversion to shared memory would cost more than the bytes allow.
+// At most 16 rows (queries x heads of a group) a CTA. Bound by the bytes of the cache, 2 (D + 4) a
+// key, as long as the instructions for them fit under the copies. So the tensor work runs on
+// warp-wide products that take the codes straight from registers (two codes to fp16 in one
+// instruction), and the rows are the products' narrow side: S^T = K Q^T and O^T = V^T P^T, 16 keys or
+// 16 columns by 8 rows a product, so that 1 to 8 rows waste half of what 16-row tiles would.
+// Every warp streams its own 32-key groups through its own ring of asynchronous copies (no barrier
+// between warps) and keeps its own running max, sum and output; the four warps are merged once at
+// the end. A 128-row tile would be 1/16 full and the way through shared memory and TMEM would cost
+// more than the bytes. (Warp-wide e4m3 products are no way around the conversion: on sm_100 they run
+// as conversions and fp16 products themselves; measured 162 against 137 us.)
 //
-// Operand layouts. The products sum over d (QK^T) and over keys (PV) in any order, so both
-// operands use the order in which a lane's bytes lie in memory: in QK^T lane (g, c) = (lane / 4,
-// lane % 4) reads D / 4 contiguous bytes of key g's row, four to a 16-wide step; in PV it reads D / 8
-// contiguous bytes at column g D / 8 of the keys 2c, 2c + 1, 2c + 8, 2c + 9 and interleaves pairs of
-// keys, so its sums hold 2 x D / 8 contiguous output columns.
+// Operand layouts, lane (g, c) = (lane / 4, lane % 4). The products sum over d (QK^T) and over keys
+// (PV) in any order, so both operands use the order in which a lane's bytes lie in memory: for QK^T
+// a lane reads D / 4 contiguous bytes of the keys g and g + 8, four to a 16-wide step; for PV D / 8
+// contiguous bytes at column g D / 8 of the keys 2c, 2c + 1, 2c + 8, 2c + 9, and interleaves pairs of
+// keys, so it holds D / 8 contiguous output columns of the rows 2c and 2c + 1. P^T comes out of the
+// first product with a lane's keys g, g + 8 and is turned by 8 x 8 transposes.
 
 constexpr int DEC_WARPS = 4;
-constexpr int DEC_STAGES = 4;
+constexpr int DEC_KEYS = 32;   // of a group
+constexpr int DEC_STAGES = 2;  // 12 warps an SM x one group on its way: 96 KB
 
 template <int D>
 struct Dec {
-  static constexpr int ROW = D;                       // bytes of a row of codes
-  static constexpr int STAGE = 2 * 16 * ROW + 128;    // K, V codes of 16 keys, their scales
-  static constexpr int RING = DEC_STAGES * STAGE;     // a warp's ring, later its output (64 D bytes)
+  static constexpr int PIECES = D / 16;                    // 16-byte pieces of a row of codes
+  static constexpr int CODES = DEC_KEYS * D;               // bytes of a group's K (or V) codes
+  static constexpr int STAGE = 2 * CODES + 2 * DEC_KEYS * 4;  // and the scales
+  static constexpr int OUT = 16 * (D + 4) * 4;             // the warp's output, later, in the same place
+  static constexpr int RING = DEC_STAGES * STAGE > OUT ? DEC_STAGES * STAGE : OUT;
   static constexpr int SMEM = DEC_WARPS * RING + DEC_WARPS * 2 * 16 * 4;
-  static_assert(RING >= 16 * D * 4, "the ring is reused for the warp's output");
   // 16-byte pieces of a row are stored at piece ^ swz(row): spreads the lanes' reads over the banks.
-  __device__ static int swz_k(int row) { return D == 128 ? (row & 1) << 2 : 0; }
-  __device__ static int swz_v(int row) { return D == 128 ? row & 6 : D == 64 ? (row >> 1) & 3 : 0; }
+  __device__ static constexpr int swz_k(int row) { return D == 128 ? (row & 1) << 2 : 0; }
+  __device__ static constexpr int swz_v(int row) { return D == 128 ? row & 6 : D == 64 ? (row >> 1) & 3 : 0; }
 };
 
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+// c += a * b, fp16 operands, 16 x 8 x 16.
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
+}
+__device__ __forceinline__ uint32_t f16_lo(uint32_t w) { return f16x2_of_e4m3x2(static_cast<uint16_t>(w)); }
+__device__ __forceinline__ uint32_t f16_hi(uint32_t w) { return f16x2_of_e4m3x2(static_cast<uint16_t>(w >> 16)); }
 
 // N bytes (2, 4, 8, 16) of shared memory into words.
 template <int N>
@@ -61,18 +76,23 @@ __device__ __forceinline__ void lds(uint32_t addr, uint32_t* w) {
   }
 }
 
-__device__ __forceinline__ float quad_max(float x) {
-  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-  return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+// Over the lanes of one c: the keys of a row.
+__device__ __forceinline__ float keys_max(float x) {
+  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+  return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
 }
-__device__ __forceinline__ float quad_sum(float x) {
-  x += __shfl_xor_sync(0xffffffffu, x, 1);
-  return x + __shfl_xor_sync(0xffffffffu, x, 2);
+__device__ __forceinline__ float keys_sum(float x) {
+  x += __shfl_xor_sync(0xffffffffu, x, 4);
+  x += __shfl_xor_sync(0xffffffffu, x, 8);
+  return x + __shfl_xor_sync(0xffffffffu, x, 16);
 }
 
-template <int D, bool BF16>
-__global__ void __launch_bounds__(DEC_WARPS * 32) decode_kernel(const AttnArgs a) {
+// NT: 8-row tiles of the row block (1 or 2).
+template <int D, bool BF16, int NT>
+__global__ void __launch_bounds__(DEC_WARPS * 32, 3) decode_kernel(const AttnArgs a) {
   using C = Dec<D>;
+  constexpr int ROWS = 8 * NT;
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
@@ -84,69 +104,97 @@ __global__ void __launch_bounds__(DEC_WARPS * 32) decode_kernel(const AttnArgs a
   x /= a.splits;
   const int h = x % a.heads_kv, b = x / a.heads_kv;
   const Seq sq = sequence(a, b);
-  const int rows = sq.n_q * a.group, row0 = rb * 16;
+  const int rows = sq.n_q * a.group, row0 = rb * ROWS;
   if (row0 >= rows) return;
-  const int kend = keys_end(a, sq, row0, min(16, rows - row0));
+  const int kend = keys_end(a, sq, row0, min(ROWS, rows - row0));
   const int k0 = split * a.split_keys;
   const int k1 = min(kend, k0 + a.split_keys);
   if (k1 <= k0 && a.splits > 1) return;  // the merge kernel does not read this split
 
   const uint32_t ring = fa2::smem_u32(smem) + warp * C::RING;
-  const int n_groups = k1 > k0 ? (k1 - k0 + 15) / 16 : 0;
+  const int n_groups = k1 > k0 ? (k1 - k0 + DEC_KEYS - 1) / DEC_KEYS : 0;
   const int mine = n_groups > warp ? (n_groups - warp + DEC_WARPS - 1) / DEC_WARPS : 0;
   const int* bt = a.bt + b * a.bt_stride;
-  const uint8_t* kh = a.c.k + h * a.c.k_st[2];
-  const uint8_t* vh = a.c.v + h * a.c.v_st[2];
+  // A lane copies piece lane % PIECES of the rows lane / PIECES + STEP * i of a group, and the scales
+  // of key `lane`.
+  constexpr int STEP = 32 / C::PIECES;
+  const int my_row = lane / C::PIECES, my_piece = lane % C::PIECES;
+  const uint8_t* kh = a.c.k + h * a.c.k_st[2] + my_piece * 16;
+  const uint8_t* vh = a.c.v + h * a.c.v_st[2] + my_piece * 16;
   const float* ksh = a.c.ks + h * a.c.ks_st[2];
   const float* vsh = a.c.vs + h * a.c.vs_st[2];
-  auto group_pos = [&](int it) { return k0 + 16 * (warp + DEC_WARPS * it); };
-  // A 16-key group lies in one page. Its table entry is fetched one group ahead.
-  int next_page = mine > 0 ? __ldg(bt + page_of(a.c, group_pos(0))) : 0;
+  auto group_pos = [&](int it) { return k0 + DEC_KEYS * (warp + DEC_WARPS * it); };
+  // Each half of a group, 16 keys, lies in one page. The table entries are fetched a group ahead.
+  auto page_at = [&](int it, int half) -> int {
+    const int pos = group_pos(it) + 16 * half;
+    return it < mine && pos < sq.len ? __ldg(bt + page_of(a.c, pos)) : 0;
+  };
+  int next_page[2] = {page_at(0, 0), page_at(0, 1)};
   auto issue = [&](int it) {
     if (it < mine) {
       const int pos0 = group_pos(it);
-      const int64_t page = next_page;
-      if (it + 1 < mine) next_page = __ldg(bt + page_of(a.c, group_pos(it + 1)));
-      const int r0 = pos0 - page_of(a.c, pos0) * a.c.page_size;
+      const int page[2] = {next_page[0], next_page[1]};
+      next_page[0] = page_at(it + 1, 0);
+      next_page[1] = page_at(it + 1, 1);
       const uint32_t st = ring + (it % DEC_STAGES) * C::STAGE;
-      const bool ok = page >= 0 && page < a.c.num_pages;
-      if (!ok) report(a.err, FA2_ERR_PAGE);
-      const int64_t pg = ok ? page : 0;
-      constexpr int PIECES = D / 16;  // of a row
+      const bool good[2] = {page[0] >= 0 && page[0] < a.c.num_pages, page[1] >= 0 && page[1] < a.c.num_pages};
+      if (!good[0] || !good[1]) report(a.err, FA2_ERR_PAGE);
+      const uint32_t sc = st + 2 * C::CODES + lane * 4;
+      const bool full = good[0] && good[1] && pos0 + DEC_KEYS <= sq.len;
 #pragma unroll
-      for (int i = 0; i < (16 * PIECES + 31) / 32; ++i) {
-        const int e = i * 32 + lane;
-        const int r = e / PIECES, piece = e % PIECES;
-        if (16 * PIECES % 32 == 0 || e < 16 * PIECES) {
-          const bool in = ok && pos0 + r < sq.len;  // rows past the end hold anything: zeros instead
-          cp_async16(st + r * C::ROW + ((piece ^ C::swz_k(r)) << 4),
-                     kh + pg * a.c.k_st[0] + (in ? r0 + r : 0) * a.c.k_st[1] + piece * 16, in);
-          cp_async16(st + 16 * C::ROW + r * C::ROW + ((piece ^ C::swz_v(r)) << 4),
-                     vh + pg * a.c.v_st[0] + (in ? r0 + r : 0) * a.c.v_st[1] + piece * 16, in);
+      for (int z = 0; z < 2; ++z) {  // 16 keys of one page
+        const int pos = pos0 + 16 * z, pg = good[z] ? page[z] : 0;
+        const int r = pos - page_of(a.c, pos) * a.c.page_size;
+        const uint8_t* kp = kh + (static_cast<int64_t>(pg) * a.c.k_page16 << 4);
+        const uint8_t* vp = vh + (static_cast<int64_t>(pg) * a.c.v_page16 << 4);
+        if constexpr (STEP <= 16) {
+          kp += static_cast<int64_t>(r + my_row) * a.c.k_row;
+          vp += static_cast<int64_t>(r + my_row) * a.c.v_row;
+#pragma unroll
+          for (int i = 0; i < 16 / STEP; ++i) {
+            const int row = 16 * z + i * STEP + my_row;
+            const uint32_t dk = st + row * D + ((my_piece ^ C::swz_k(row)) << 4);
+            const uint32_t dv = st + C::CODES + row * D + ((my_piece ^ C::swz_v(row)) << 4);
+            if (full) {
+              cp_async16_full(dk, kp + static_cast<int64_t>(i * STEP) * a.c.k_row);
+              cp_async16_full(dv, vp + static_cast<int64_t>(i * STEP) * a.c.v_row);
+            } else {  // rows past the end or of a refused page hold anything: zeros instead
+              const bool in = good[z] && pos0 + row < sq.len;
+              cp_async16(dk, in ? kp + static_cast<int64_t>(i * STEP) * a.c.k_row : kh, in);
+              cp_async16(dv, in ? vp + static_cast<int64_t>(i * STEP) * a.c.v_row : vh, in);
+            }
+          }
+        } else if (my_row / 16 == z) {  // D = 16: 32 rows at once
+          const int64_t rr = r + (my_row & 15);
+          const bool in = good[z] && pos0 + my_row < sq.len;
+          cp_async16(st + my_row * D, in ? kp + rr * a.c.k_row : kh, in);
+          cp_async16(st + C::CODES + my_row * D, in ? vp + rr * a.c.v_row : vh, in);
         }
-      }
-      const int r = lane & 15;
-      const bool in = ok && pos0 + r < sq.len;
-      const float* src = lane < 16 ? ksh + pg * a.c.ks_st[0] + (in ? r0 + r : 0) * a.c.ks_st[1]
-                                   : vsh + pg * a.c.vs_st[0] + (in ? r0 + r : 0) * a.c.vs_st[1];
-      const uint32_t dst = st + 32 * C::ROW + lane * 4;
-      if (ok) {
-        cp_async4(dst, src, in);
-      } else {  // a refused page: queries that see its keys get NaN
-        asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst), "r"(0x7fc00000u) : "memory");
+        if (lane / 16 == z) {
+          const int64_t rr = r + (lane & 15);
+          const bool in = good[z] && pos0 + lane < sq.len;
+          if (good[z]) {
+            cp_async4(sc, in ? ksh + static_cast<int64_t>(pg) * a.c.ks_page + rr * a.c.ks_row : ksh, in);
+            cp_async4(sc + DEC_KEYS * 4, in ? vsh + static_cast<int64_t>(pg) * a.c.vs_page + rr * a.c.vs_row : vsh, in);
+          } else {  // a refused page: queries that see its keys get NaN
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(sc), "r"(0x7fc00000u) : "memory");
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(sc + DEC_KEYS * 4), "r"(0u) : "memory");
+          }
+        }
       }
     }
     cp_async_commit();  // also where there is nothing: the group count stays in step
   };
-  for (int it = 0; it < DEC_STAGES - 1; ++it) issue(it);
-
-  // Q, scaled by a power of two, in the order described above: this lane's rows are g and g + 8.
-  uint32_t qa[D / 16][4];
-  float row_sc[2];
-  int lim[2];
 #pragma unroll
-  for (int rr = 0; rr < 2; ++rr) {
-    const int row = row0 + g + 8 * rr;
+  for (int it = 0; it < DEC_STAGES; ++it) issue(it);
+
+  // Q: this lane holds values of the rows 8 t + g, in the order described above, times the power of
+  // two that brings the row's largest value below 2^15 (exact in fp16).
+  uint32_t qb[NT][D / 16][2];
+  __shared__ float q_scale[DEC_WARPS][16];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int row = row0 + 8 * t + g;
     constexpr int NB = D >= 64 ? 16 : D / 4;  // values of a contiguous piece
     uint32_t w[D / 8];                        // D / 4 values
     uint32_t top = 0;
@@ -154,10 +202,10 @@ __global__ void __launch_bounds__(DEC_WARPS * 32) decode_kernel(const AttnArgs a
     const uint16_t* src = q_row(a, sq, b, h, in ? row : row0);
 #pragma unroll
     for (int p = 0; p < D / 4 / NB; ++p) {
-      const uint16_t* s = src + p * 64 + c * NB;
+      const uint32_t* s = reinterpret_cast<const uint32_t*>(src + p * 64 + c * NB);
 #pragma unroll
       for (int i = 0; i < NB / 2; ++i) {
-        w[p * NB / 2 + i] = in ? *reinterpret_cast<const uint32_t*>(s + 2 * i) : 0;
+        w[p * NB / 2 + i] = in ? __ldg(s + i) : 0u;
         const float2 v = float2_of_x2<BF16>(w[p * NB / 2 + i]);
         top = max(top, max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu));
       }
@@ -165,224 +213,289 @@ __global__ void __launch_bounds__(DEC_WARPS * 32) decode_kernel(const AttnArgs a
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const int e = row_exponent(top);
-    const float f = pow2f(14 - e);
-    row_sc[rr] = a.qk_scale * pow2f(max(-126, e - 14));
+    const float f = top < 0x7f800000u ? pow2f(14 - e) : __uint_as_float(0x7fc00000u);  // NaN, infinity: a NaN row
+    if (c == 0) q_scale[warp][8 * t + g] = a.qk_scale * pow2f(max(-126, e - 14));
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) {
       const float2 lo = float2_of_x2<BF16>(w[2 * s]), hi = float2_of_x2<BF16>(w[2 * s + 1]);
-      qa[s][rr] = x2_of_floats<false>(lo.x * f, lo.y * f);
-      qa[s][2 + rr] = x2_of_floats<false>(hi.x * f, hi.y * f);
+      qb[t][s][0] = x2_of_floats<false>(lo.x * f, lo.y * f);
+      qb[t][s][1] = x2_of_floats<false>(hi.x * f, hi.y * f);
     }
-    lim[rr] = in ? last_key(a, sq, row / a.group) : -1;
+  }
+  __syncwarp();
+  // From here on this lane's rows are 8 t + 2c + i.
+  float row_sc[NT][2], m[NT][2], l[NT][2];
+  int lim[NT][2];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = 8 * t + 2 * c + i;
+      row_sc[t][i] = q_scale[warp][r];
+      lim[t][i] = row0 + r < rows ? last_key(a, sq, (row0 + r) / a.group) : -1;
+      m[t][i] = -INFINITY;
+      l[t][i] = 0.0f;
+    }
   }
   const int lim_first = last_key(a, sq, row0 / a.group);  // the smallest of the block's rows
 
-  float o[D / 8][4];
+  float o[NT][D / 16][4];
 #pragma unroll
-  for (int j = 0; j < D / 8; ++j) {
+  for (int t = 0; t < NT; ++t) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[j][i] = 0.0f;
+    for (int j = 0; j < D / 16; ++j) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[t][j][i] = 0.0f;
+    }
   }
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
   int eb = EB_MIN;  // exponent field of the largest finite sv so far
+  constexpr int HALVES = DEC_KEYS / 16;
 
   for (int it = 0; it < mine; ++it) {
-    issue(it + DEC_STAGES - 1);
     cp_async_wait<DEC_STAGES - 1>();
     __syncwarp();
     const uint32_t st = ring + (it % DEC_STAGES) * C::STAGE;
     const int pos0 = group_pos(it);
 
-    float s[2][4] = {};
+    // Scores: s[t][z][0..3] = (key 16 z + g, rows 8 t + 2c, + 1), (key 16 z + g + 8, the same rows).
+    float s[NT][HALVES][4];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int r = t * 8 + g;
+    for (int z = 0; z < HALVES; ++z) {
+      const int r = 16 * z + g;
       constexpr int NB = D >= 64 ? 16 : D / 4;
 #pragma unroll
+      for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[t][z][i] = 0.0f;
+      }
+#pragma unroll
       for (int p = 0; p < D / 4 / NB; ++p) {
-        uint32_t w[4];
+        uint32_t w0[4], w1[4];
         const int byte = p * 64 + c * NB;
-        lds<NB>(st + r * C::ROW + (((byte >> 4) ^ C::swz_k(r)) << 4) + (byte & 15), w);
+        lds<NB>(st + r * D + (((byte >> 4) ^ C::swz_k(r)) << 4) + (byte & 15), w0);
+        lds<NB>(st + (r + 8) * D + (((byte >> 4) ^ C::swz_k(r + 8)) << 4) + (byte & 15), w1);
 #pragma unroll
         for (int i = 0; i < NB / 4; ++i) {
-          mma16816(s[t], qa[p * 4 + i], f16x2_of_e4m3x2(static_cast<uint16_t>(w[i])),
-                   f16x2_of_e4m3x2(static_cast<uint16_t>(w[i] >> 16)));
+          const uint32_t a0 = f16_lo(w0[i]), a1 = f16_lo(w1[i]), a2 = f16_hi(w0[i]), a3 = f16_hi(w1[i]);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) mma_f16(s[t][z], a0, a1, a2, a3, qb[t][p * 4 + i][0], qb[t][p * 4 + i][1]);
         }
       }
     }
-    // Scales of this lane's keys: 2c, 2c + 1 (tile 0) and 8 + 2c, 8 + 2c + 1 (tile 1).
-    float sk[2][2], sv[2][2];
+    // Scales of this lane's keys: 16 z + 8 y + g.
+    float sk[HALVES][2], sv[HALVES][2];
+    uint32_t top = 0;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      uint32_t w[2];
-      lds<8>(st + 32 * C::ROW + (t * 8 + 2 * c) * 4, w);
-      sk[t][0] = __uint_as_float(w[0]);
-      sk[t][1] = __uint_as_float(w[1]);
-      lds<8>(st + 32 * C::ROW + 64 + (t * 8 + 2 * c) * 4, w);
-      sv[t][0] = __uint_as_float(w[0]);
-      sv[t][1] = __uint_as_float(w[1]);
+    for (int z = 0; z < HALVES; ++z) {
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        uint32_t w;
+        lds<4>(st + 2 * C::CODES + (16 * z + 8 * y + g) * 4, &w);
+        sk[z][y] = __uint_as_float(w);
+        lds<4>(st + 2 * C::CODES + (DEC_KEYS + 16 * z + 8 * y + g) * 4, &w);
+        sv[z][y] = __uint_as_float(w);
+        top = max(top, w & 0x7fffffffu);
+      }
     }
-    uint32_t sv_top = 0;
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (top >= 0x7f800000u) {
+      // A value row that is not finite makes its key's score NaN instead (0 * NaN in the second
+      // product would reach the rows that do not see the key).
+      top = 0;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+      for (int z = 0; z < HALVES; ++z) {
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          if (!(fabsf(sv[z][y]) < INFINITY)) {
+            sk[z][y] = __uint_as_float(0x7fc00000u);
+            sv[z][y] = 0.0f;
+          }
+          top = max(top, __float_as_uint(sv[z][y]) & 0x7fffffffu);
+        }
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
+    }
+    const bool masked = pos0 + DEC_KEYS - 1 > lim_first;
+    const int eb_new = max(eb, static_cast<int>(top >> 23));  // the same in every lane
+    bool bump = eb_new > eb;
+    float cand[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int z = 0; z < HALVES; ++z) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[t][z][i] *= sk[z][i >> 1];
+      }
+      if (masked) {
+#pragma unroll
+        for (int z = 0; z < HALVES; ++z) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (pos0 + 16 * z + 8 * (i >> 1) + g > lim[t][i & 1]) s[t][z][i] = -INFINITY;
+          }
+        }
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const uint32_t v = __float_as_uint(sv[t][i]) & 0x7fffffffu;
-        sv_top = max(sv_top, v < 0x7f800000u ? v : 0u);
+        float v = fmaxf(s[t][0][i], s[t][0][i + 2]);
+#pragma unroll
+        for (int z = 1; z < HALVES; ++z) v = fa2::fmax3(v, s[t][z][i], s[t][z][i + 2]);
+        cand[t][i] = keys_max(v) * row_sc[t][i];
+        bump = bump || cand[t][i] > m[t][i] + RESCALE_TH;
       }
     }
-    sv_top = max(sv_top, __shfl_xor_sync(0xffffffffu, sv_top, 1));
-    sv_top = max(sv_top, __shfl_xor_sync(0xffffffffu, sv_top, 2));
-
-    const bool masked = pos0 + 15 > lim_first || row0 + 16 > rows;
-    float cand[2];
-#pragma unroll
-    for (int rr = 0; rr < 2; ++rr) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float v = s[t][2 * rr + i] * sk[t][i];
-          if (masked && pos0 + t * 8 + 2 * c + i > lim[rr]) v = -INFINITY;
-          s[t][2 * rr + i] = v;
-        }
-      }
-      cand[rr] = quad_max(fmaxf(fmaxf(s[0][2 * rr], s[0][2 * rr + 1]), fmaxf(s[1][2 * rr], s[1][2 * rr + 1]))) * row_sc[rr];
-    }
-    const int eb_new = max(eb, static_cast<int>(sv_top >> 23));  // the same in every lane
-    const bool bump = cand[0] > m[0] + RESCALE_TH || cand[1] > m[1] + RESCALE_TH || eb_new > eb;
     if (__any_sync(0xffffffffu, bump)) {
       const float fe = eb_new - eb > 126 ? 0.0f : pow2f(eb - eb_new);
-      float al[2];
 #pragma unroll
-      for (int rr = 0; rr < 2; ++rr) {
-        al[rr] = 1.0f;
-        if (cand[rr] > m[rr] + RESCALE_TH) {
-          al[rr] = fa2::ex2_mufu(m[rr] - cand[rr]);  // 0 the first time (m = -inf)
-          m[rr] = cand[rr];
+      for (int t = 0; t < NT; ++t) {
+        float al[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          al[i] = 1.0f;
+          if (cand[t][i] > m[t][i] + RESCALE_TH) {
+            al[i] = fa2::ex2_mufu(m[t][i] - cand[t][i]);  // 0 the first time (m = -inf)
+            m[t][i] = cand[t][i];
+          }
+          l[t][i] *= al[i];
+          al[i] *= fe;
         }
-        l[rr] *= al[rr];
-        al[rr] *= fe;
-      }
 #pragma unroll
-      for (int j = 0; j < D / 8; ++j) {
-        o[j][0] *= al[0];
-        o[j][1] *= al[0];
-        o[j][2] *= al[1];
-        o[j][3] *= al[1];
+        for (int j = 0; j < D / 16; ++j) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[t][j][i] *= al[i & 1];
+        }
       }
       eb = eb_new;
     }
     const float gs = __uint_as_float(static_cast<uint32_t>(254 + P_SHIFT - eb) << 23);
-    uint32_t pa[4];
+    uint32_t pb[NT][HALVES][2];
 #pragma unroll
-    for (int rr = 0; rr < 2; ++rr) {
-      const float mr = m[rr] == -INFINITY ? 0.0f : m[rr];
+    for (int z = 0; z < HALVES; ++z) {
+      sv[z][0] *= gs;
+      sv[z][1] *= gs;
+    }
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        float p[2], w[2];
+    for (int t = 0; t < NT; ++t) {
+      const float m0 = m[t][0] == -INFINITY ? 0.0f : m[t][0], m1 = m[t][1] == -INFINITY ? 0.0f : m[t][1];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float v = s[t][2 * rr + i];
-          p[i] = fa2::ex2_mufu(fmaf(v, row_sc[rr], -mr));
-          // A masked key's scale may be anything: its weight is 0, not 0 * sv.
-          w[i] = masked && pos0 + t * 8 + 2 * c + i > lim[rr] ? 0.0f : p[i] * (sv[t][i] * gs);
+      for (int z = 0; z < HALVES; ++z) {
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const float p0 = fa2::ex2_mufu(fmaf(s[t][z][2 * y], row_sc[t][0], -m0));
+          const float p1 = fa2::ex2_mufu(fmaf(s[t][z][2 * y + 1], row_sc[t][1], -m1));
+          l[t][0] += p0;
+          l[t][1] += p1;
+          pb[t][z][y] = transpose8x8(x2_of_floats<false>(p0 * sv[z][y], p1 * sv[z][y]));
         }
-        l[rr] += p[0] + p[1];
-        pa[rr + 2 * t] = x2_of_floats<false>(w[0], w[1]);
       }
     }
-    // O += P' V.
-    uint32_t v0[4], v1[4], v2[4], v3[4];
-    {
+    // O^T += V^T P'^T, 16 keys at a time.
+#pragma unroll
+    for (int z = 0; z < HALVES; ++z) {
+      uint32_t v0[4], v1[4], v2[4], v3[4];
       constexpr int NB = D / 8;
       const int byte = g * NB;
-      const uint32_t vst = st + 16 * C::ROW;
-      auto at = [&](int r) { return vst + r * C::ROW + (((byte >> 4) ^ C::swz_v(r)) << 4) + (byte & 15); };
-      lds<NB>(at(2 * c), v0);
-      lds<NB>(at(2 * c + 1), v1);
-      lds<NB>(at(2 * c + 8), v2);
-      lds<NB>(at(2 * c + 9), v3);
-    }
+      const uint32_t vst = st + C::CODES;
+      auto at = [&](int r) { return vst + r * D + (((byte >> 4) ^ C::swz_v(r)) << 4) + (byte & 15); };
+      lds<NB>(at(16 * z + 2 * c), v0);
+      lds<NB>(at(16 * z + 2 * c + 1), v1);
+      lds<NB>(at(16 * z + 2 * c + 8), v2);
+      lds<NB>(at(16 * z + 2 * c + 9), v3);
 #pragma unroll
-    for (int w = 0; w < (D + 31) / 32; ++w) {
-      const uint32_t e0 = __byte_perm(v0[w], v1[w], 0x5140), e1 = __byte_perm(v2[w], v3[w], 0x5140);
-      mma16816(o[4 * w], pa, f16x2_of_e4m3x2(static_cast<uint16_t>(e0)), f16x2_of_e4m3x2(static_cast<uint16_t>(e1)));
-      mma16816(o[4 * w + 1], pa, f16x2_of_e4m3x2(static_cast<uint16_t>(e0 >> 16)), f16x2_of_e4m3x2(static_cast<uint16_t>(e1 >> 16)));
-      if constexpr (D >= 32) {
-        const uint32_t f0 = __byte_perm(v0[w], v1[w], 0x7362), f1 = __byte_perm(v2[w], v3[w], 0x7362);
-        mma16816(o[4 * w + 2], pa, f16x2_of_e4m3x2(static_cast<uint16_t>(f0)), f16x2_of_e4m3x2(static_cast<uint16_t>(f1)));
-        mma16816(o[4 * w + 3], pa, f16x2_of_e4m3x2(static_cast<uint16_t>(f0 >> 16)), f16x2_of_e4m3x2(static_cast<uint16_t>(f1 >> 16)));
+      for (int w = 0; w < (D + 31) / 32; ++w) {
+        const uint32_t e0 = __byte_perm(v0[w], v1[w], 0x5140), e1 = __byte_perm(v2[w], v3[w], 0x5140);
+        const uint32_t a0 = f16_lo(e0), a1 = f16_hi(e0), a2 = f16_lo(e1), a3 = f16_hi(e1);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) mma_f16(o[t][2 * w], a0, a1, a2, a3, pb[t][z][0], pb[t][z][1]);
+        if constexpr (D >= 32) {
+          const uint32_t f0 = __byte_perm(v0[w], v1[w], 0x7362), f1 = __byte_perm(v2[w], v3[w], 0x7362);
+          const uint32_t c0 = f16_lo(f0), c1 = f16_hi(f0), c2 = f16_lo(f1), c3 = f16_hi(f1);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) mma_f16(o[t][2 * w + 1], c0, c1, c2, c3, pb[t][z][0], pb[t][z][1]);
+        }
       }
     }
     __syncwarp();  // every lane has read the stage before it is filled again
+    issue(it + DEC_STAGES);
   }
   cp_async_wait<0>();
   __syncwarp();
 
-  // Merge the warps: (m, l, O) of each in shared memory, O in the sv's own units.
+  // Merge the warps: (m, l, O) of each in shared memory, O in the sv's own units. Rows of O are D + 4
+  // floats apart: the four rows that the lanes of one g write lie in different banks.
   float* wo = reinterpret_cast<float*>(smem + warp * C::RING);
   float* wm = reinterpret_cast<float*>(smem + DEC_WARPS * C::RING);  // [warp][16]
   float* wl = wm + DEC_WARPS * 16;
   // 2^(eb - 127 - P_SHIFT), as two factors so that neither leaves the normal range.
-  const float u0 = pow2f((eb - 127 - P_SHIFT) / 2), u1 = pow2f((eb - 127 - P_SHIFT) - (eb - 127 - P_SHIFT) / 2);
+  const int ex = eb - 127 - P_SHIFT;
+  const float u0 = pow2f(ex / 2), u1 = pow2f(ex - ex / 2);
 #pragma unroll
-  for (int rr = 0; rr < 2; ++rr) {
-    const float sum = quad_sum(l[rr]);
-    const int r = g + 8 * rr;
-    if (c == 0) {
-      wm[warp * 16 + r] = m[rr];
-      wl[warp * 16 + r] = sum;
-    }
+  for (int t = 0; t < NT; ++t) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      float* dst = wo + r * D + (2 * c + i) * (D / 8);
+      const float sum = keys_sum(l[t][i]);
+      const int r = 8 * t + 2 * c + i;
+      if (g == 0) {
+        wm[warp * 16 + r] = m[t][i];
+        wl[warp * 16 + r] = sum;
+      }
+      float* dst = wo + r * (D + 4) + g * (D / 8);
 #pragma unroll
-      for (int j = 0; j < D / 8; ++j) dst[j] = o[j][2 * rr + i] * u0 * u1;
+      for (int j = 0; j < D / 16; ++j) {
+        *reinterpret_cast<float2*>(dst + 2 * j) = make_float2(o[t][j][i] * u0 * u1, o[t][j][2 + i] * u0 * u1);
+      }
     }
   }
   __syncthreads();
-  const int r = threadIdx.x >> 3, part = threadIdx.x & 7;  // 128 threads: 16 rows x 8 parts
+  constexpr int PARTS = DEC_WARPS * 32 / ROWS;  // threads of a row
+  const int r = static_cast<int>(threadIdx.x) / PARTS, part = static_cast<int>(threadIdx.x) % PARTS;
   const int row = row0 + r;
   if (row >= rows) return;
-  constexpr int PER = D / 8;
   float mx = -INFINITY;
 #pragma unroll
   for (int w = 0; w < DEC_WARPS; ++w) mx = fmaxf(mx, wm[w * 16 + r]);
-  float sum = 0.0f, acc[PER];
-#pragma unroll
-  for (int j = 0; j < PER; ++j) acc[j] = 0.0f;
+  float sum = 0.0f, f[DEC_WARPS];
 #pragma unroll
   for (int w = 0; w < DEC_WARPS; ++w) {
     const float mw = wm[w * 16 + r], lw = wl[w * 16 + r];
     // A warp that saw no key of the row has m = -inf and l = 0; a NaN sum is kept.
-    const float f = mw == -INFINITY ? (lw == 0.0f ? 0.0f : 1.0f) : exp2f(mw - mx);
-    if (f == 0.0f) continue;
-    sum = fmaf(f, lw, sum);
-    const float* src = reinterpret_cast<const float*>(smem + w * C::RING) + r * D + part * PER;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) acc[j] = fmaf(f, src[j], acc[j]);
+    f[w] = mw == -INFINITY ? (lw == 0.0f ? 0.0f : 1.0f) : exp2f(mw - mx);
+    sum = f[w] == 0.0f ? sum : fmaf(f[w], lw, sum);
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const int64_t slot = (static_cast<int64_t>(b * a.heads_kv + h) * a.splits + split) * a.rows_pad + row;
+  constexpr int PER = D / PARTS > 0 ? (D / PARTS < 8 ? D / PARTS : 8) : 1;  // neighbouring columns at a time
+  for (int d = part * PER; d < D; d += PARTS * PER) {
+    float acc[PER] = {};
 #pragma unroll
-  for (int j = 0; j < PER; ++j) acc[j] *= inv;
-  if (a.splits > 1) {
-    const int64_t slot = (static_cast<int64_t>(b * a.heads_kv + h) * a.splits + split) * a.rows_pad + row;
-    float* dst = a.o_part + slot * D + part * PER;
+    for (int w = 0; w < DEC_WARPS; ++w) {
+      if (f[w] == 0.0f) continue;
+      const float* src = reinterpret_cast<const float*>(smem + w * C::RING) + r * (D + 4) + d;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) dst[j] = acc[j];
-    if (part == 0) a.lse_part[slot] = sum == 0.0f ? -INFINITY : (mx == -INFINITY ? 0.0f : mx) + log2f(sum);
-  } else {
-    uint32_t* dst = reinterpret_cast<uint32_t*>(o_row(a, sq, b, h, row) + part * PER);
+      for (int j = 0; j < PER; ++j) acc[j] = fmaf(f[w], src[j], acc[j]);
+    }
+    if (a.splits > 1) {
 #pragma unroll
-    for (int j = 0; j < PER; j += 2) dst[j / 2] = x2_of_floats<BF16>(acc[j], acc[j + 1]);
+      for (int j = 0; j < PER; ++j) a.o_part[slot * D + d + j] = acc[j] * inv;
+    } else {
+      uint16_t* dst = o_row(a, sq, b, h, row) + d;
+      if constexpr (PER >= 2) {
+#pragma unroll
+        for (int j = 0; j < PER; j += 2) {
+          *reinterpret_cast<uint32_t*>(dst + j) = x2_of_floats<BF16>(acc[j] * inv, acc[j + 1] * inv);
+        }
+      } else {
+        dst[0] = x1_of_float<BF16>(acc[0] * inv);
+      }
+    }
   }
+  if (a.splits > 1 && part == 0) a.lse_part[slot] = sum == 0.0f ? -INFINITY : (mx == -INFINITY ? 0.0f : mx) + log2f(sum);
 }
 
 // ------------------------------------------------------------------ merge of the key ranges
 // One warp a row: o = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max) in split order.
-template <int D, bool BF16, int ROWS>
-__global__ void __launch_bounds__(128) merge_kernel(const AttnArgs a) {
+template <int D, bool BF16>
+__global__ void __launch_bounds__(128) merge_kernel(const AttnArgs a, int block) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t x = static_cast<int64_t>(blockIdx.x) * 4 + warp;
   const int row = static_cast<int>(x % a.rows_pad);
@@ -392,8 +505,8 @@ __global__ void __launch_bounds__(128) merge_kernel(const AttnArgs a) {
   const Seq sq = sequence(a, b);
   const int rows = sq.n_q * a.group;
   if (row >= rows) return;
-  const int row0 = row / ROWS * ROWS;
-  const int ns = (keys_end(a, sq, row0, min(ROWS, rows - row0)) + a.split_keys - 1) / a.split_keys;
+  const int row0 = row / block * block;
+  const int ns = (keys_end(a, sq, row0, min(block, rows - row0)) + a.split_keys - 1) / a.split_keys;
   const float* lse = a.lse_part + static_cast<int64_t>(bh) * a.splits * a.rows_pad + row;
   const float* op = a.o_part + (static_cast<int64_t>(bh) * a.splits * a.rows_pad + row) * D;
   float mx = -INFINITY;
@@ -430,7 +543,7 @@ __global__ void __launch_bounds__(128) merge_kernel(const AttnArgs a) {
 
 // ------------------------------------------------------------------------------------ host
 struct Plan {
-  bool chunk = false;  // the 256-row kernel
+  int block = 8;  // rows of a block: 8 or 16 (decode_kernel), 256 (chunk_kernel)
   int row_blocks = 1, rows_pad = 16, splits = 1, split_keys = 0;
   int64_t lse_floats = 0, bytes = 0;
 };
@@ -441,17 +554,17 @@ constexpr int MAX_SPLITS = 256;
 Plan plan(const Fa2Kv8AttnParams* p) {
   Plan r;
   const int64_t rows = static_cast<int64_t>(p->seqlen_q) * (p->heads_q / p->cache.heads_kv);
-  r.chunk = rows > 16;
-  const int per_block = r.chunk ? 256 : 16;
-  r.row_blocks = static_cast<int>((rows + per_block - 1) / per_block);
-  r.rows_pad = r.row_blocks * per_block;
+  r.block = rows <= 8 ? 8 : rows <= 16 ? 16 : 256;
+  const bool chunk = r.block == 256;
+  r.row_blocks = static_cast<int>((rows + r.block - 1) / r.block);
+  r.rows_pad = r.row_blocks * r.block;
   int64_t units = static_cast<int64_t>(p->batch) * p->cache.heads_kv * r.row_blocks;
   if (units < 1) units = 1;
-  // Few rows: one wave of three CTAs on each of 148 SMs, at least two 16-key groups for each of a
+  // Few rows: one wave of three CTAs on each of 148 SMs, at least one 32-key group for each of a
   // CTA's warps. Many rows: one wave of one CTA an SM, at least four 128-key tiles each.
-  const int unit_keys = r.chunk ? 128 : 64;
-  int64_t s = p->num_splits > 0 ? p->num_splits : (r.chunk ? 148 : 148 * 3) / units;
-  const int64_t least = p->num_splits > 0 ? unit_keys : r.chunk ? 512 : 128;
+  const int unit_keys = 128;  // one tile, or a group for each warp
+  int64_t s = p->num_splits > 0 ? p->num_splits : (chunk ? 148 : 148 * 3) / units;
+  const int64_t least = p->num_splits > 0 ? unit_keys : chunk ? 512 : 128;
   const int64_t most = (p->max_seqlen_k + least - 1) / least;
   if (s > most) s = most;
   if (s > MAX_SPLITS) s = MAX_SPLITS;
@@ -509,27 +622,26 @@ bool allow_smem(K kernel, int bytes, int dev, std::atomic<bool> (&done)[MAX_DEVI
 }
 
 template <int D, bool BF16>
-int launch(const AttnArgs& a, bool chunk, cudaStream_t s, int dev) {
-  static std::atomic<bool> done[2][MAX_DEVICES];
+int launch(const AttnArgs& a, int block, cudaStream_t s, int dev) {
+  static std::atomic<bool> done[3][MAX_DEVICES];
   const unsigned ctas = static_cast<unsigned>(static_cast<int64_t>(a.batch) * a.heads_kv * a.splits * a.row_blocks);
-  if (chunk) {
+  if (block == 256) {
     auto kernel = chunk_kernel<D, BF16>;
-    if (!allow_smem(kernel, Ch<D, BF16>::SMEM, dev, done[1])) return FA2_ERR_LAUNCH;
+    if (!allow_smem(kernel, Ch<D, BF16>::SMEM, dev, done[2])) return FA2_ERR_LAUNCH;
     kernel<<<ctas, CH_THREADS, Ch<D, BF16>::SMEM, s>>>(a);
+  } else if (block == 16) {
+    auto kernel = decode_kernel<D, BF16, 2>;
+    if (!allow_smem(kernel, Dec<D>::SMEM, dev, done[1])) return FA2_ERR_LAUNCH;
+    kernel<<<ctas, DEC_WARPS * 32, Dec<D>::SMEM, s>>>(a);
   } else {
-    auto kernel = decode_kernel<D, BF16>;
+    auto kernel = decode_kernel<D, BF16, 1>;
     if (!allow_smem(kernel, Dec<D>::SMEM, dev, done[0])) return FA2_ERR_LAUNCH;
     kernel<<<ctas, DEC_WARPS * 32, Dec<D>::SMEM, s>>>(a);
   }
   const int rc = launch_status();
   if (rc != FA2_OK || a.splits <= 1) return rc;
   const int64_t rows = static_cast<int64_t>(a.batch) * a.heads_kv * a.rows_pad;
-  const unsigned blocks = static_cast<unsigned>((rows + 3) / 4);
-  if (chunk) {
-    merge_kernel<D, BF16, 256><<<blocks, 128, 0, s>>>(a);
-  } else {
-    merge_kernel<D, BF16, 16><<<blocks, 128, 0, s>>>(a);
-  }
+  merge_kernel<D, BF16><<<static_cast<unsigned>((rows + 3) / 4), 128, 0, s>>>(a, block);
   return launch_status();
 }
 
@@ -591,10 +703,10 @@ int fa2_kv8_attn_sm100(const Fa2Kv8AttnParams* p, void* stream) {
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf = p->dtype == FA2_DTYPE_BF16;
   switch (p->cache.head_dim) {
-    case 16: return bf ? launch<16, true>(a, r.chunk, s, dev) : launch<16, false>(a, r.chunk, s, dev);
-    case 32: return bf ? launch<32, true>(a, r.chunk, s, dev) : launch<32, false>(a, r.chunk, s, dev);
-    case 64: return bf ? launch<64, true>(a, r.chunk, s, dev) : launch<64, false>(a, r.chunk, s, dev);
-    default: return bf ? launch<128, true>(a, r.chunk, s, dev) : launch<128, false>(a, r.chunk, s, dev);
+    case 16: return bf ? launch<16, true>(a, r.block, s, dev) : launch<16, false>(a, r.block, s, dev);
+    case 32: return bf ? launch<32, true>(a, r.block, s, dev) : launch<32, false>(a, r.block, s, dev);
+    case 64: return bf ? launch<64, true>(a, r.block, s, dev) : launch<64, false>(a, r.block, s, dev);
+    default: return bf ? launch<128, true>(a, r.block, s, dev) : launch<128, false>(a, r.block, s, dev);
   }
 }
 

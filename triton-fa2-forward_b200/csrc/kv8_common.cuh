@@ -23,6 +23,9 @@ struct Cache {
   int64_t k_st[3], v_st[3], ks_st[3], vs_st[3];  // (page, row, head)
   int num_pages, page_size, page_shift;           // shift >= 0 where page_size is a power of two
   int heads_kv;
+  // The same strides in 32 bits (page strides of codes in 16-byte units), for offsets that are one
+  // widening product each.
+  int k_page16, v_page16, ks_page, vs_page, k_row, v_row, ks_row, vs_row;
 };
 
 __device__ __forceinline__ int page_of(const Cache& c, int pos) {
@@ -121,7 +124,13 @@ inline int check_cache(const Fa2Kv8Cache& c) {
   }
   const int64_t n[3] = {c.num_pages, c.page_size, c.heads_kv};
   for (int i = 0; i < 3; ++i) {
-    if (n[i] > 1 && ((c.k_stride[i] | c.v_stride[i]) & 15) != 0) return FA2_ERR_LAYOUT;
+    if (n[i] <= 1) continue;  // the stride of a single entry is never used
+    if (((c.k_stride[i] | c.v_stride[i]) & 15) != 0) return FA2_ERR_LAYOUT;
+    const int64_t most = i == 0 ? 0x7fffffffll * 16 : 0x7fffffffll, most_s = 0x7fffffffll;
+    if (c.k_stride[i] < 0 || c.v_stride[i] < 0 || c.ks_stride[i] < 0 || c.vs_stride[i] < 0 || c.k_stride[i] > most ||
+        c.v_stride[i] > most || c.ks_stride[i] > most_s || c.vs_stride[i] > most_s) {
+      return FA2_ERR_LAYOUT;
+    }
   }
   return FA2_OK;
 }
@@ -145,6 +154,16 @@ inline Cache device_cache(const Fa2Kv8Cache& c) {
     if (c.page_size == (1 << s)) d.page_shift = s;
   }
   d.heads_kv = c.heads_kv;
+  if (c.num_pages > 1) {
+    d.k_page16 = static_cast<int>(c.k_stride[0] / 16);
+    d.v_page16 = static_cast<int>(c.v_stride[0] / 16);
+    d.ks_page = static_cast<int>(c.ks_stride[0]);
+    d.vs_page = static_cast<int>(c.vs_stride[0]);
+  }
+  d.k_row = static_cast<int>(c.k_stride[1]);
+  d.v_row = static_cast<int>(c.v_stride[1]);
+  d.ks_row = static_cast<int>(c.ks_stride[1]);
+  d.vs_row = static_cast<int>(c.vs_stride[1]);
   return d;
 }
 
