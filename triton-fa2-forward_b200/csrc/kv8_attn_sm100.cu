@@ -124,62 +124,78 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, 3) decode_kernel(const AttnArg
   const float* ksh = a.c.ks + h * a.c.ks_st[2];
   const float* vsh = a.c.vs + h * a.c.vs_st[2];
   auto group_pos = [&](int it) { return k0 + DEC_KEYS * (warp + DEC_WARPS * it); };
-  // Each half of a group, 16 keys, lies in one page. The table entries are fetched a group ahead.
-  auto page_at = [&](int it, int half) -> int {
-    const int pos = group_pos(it) + 16 * half;
-    return it < mine && pos < sq.len ? __ldg(bt + page_of(a.c, pos)) : 0;
+  // The next group's place: its page's index in the table, its first row there, and the page itself,
+  // fetched one group ahead. Each half of a group, 16 keys, lies in one page; both do unless pages
+  // have 16 rows. A warp's groups are 128 keys apart.
+  const bool two = a.c.page_size == 16;
+  int pi = page_of(a.c, group_pos(0)), row_in = group_pos(0) - pi * a.c.page_size;
+  int next_page[2] = {0, 0};
+  auto fetch_pages = [&](int it) {
+    if (it >= mine) return;
+    next_page[0] = next_page[1] = __ldg(bt + pi);
+    if (two && group_pos(it) + 16 < sq.len) next_page[1] = __ldg(bt + pi + 1);
   };
-  int next_page[2] = {page_at(0, 0), page_at(0, 1)};
+  fetch_pages(0);
+  // This lane's offsets within a stage and a page.
+  const uint32_t to_k = my_row * D + ((my_piece ^ C::swz_k(my_row)) << 4);
+  const uint32_t to_v = my_row * D + ((my_piece ^ C::swz_v(my_row)) << 4);
+  const int64_t step_k = static_cast<int64_t>(STEP) * a.c.k_row, step_v = static_cast<int64_t>(STEP) * a.c.v_row;
   auto issue = [&](int it) {
     if (it < mine) {
-      const int pos0 = group_pos(it);
-      const int page[2] = {next_page[0], next_page[1]};
-      next_page[0] = page_at(it + 1, 0);
-      next_page[1] = page_at(it + 1, 1);
-      const uint32_t st = ring + (it % DEC_STAGES) * C::STAGE;
-      const bool good[2] = {page[0] >= 0 && page[0] < a.c.num_pages, page[1] >= 0 && page[1] < a.c.num_pages};
-      if (!good[0] || !good[1]) report(a.err, FA2_ERR_PAGE);
-      const uint32_t sc = st + 2 * C::CODES + lane * 4;
-      const bool full = good[0] && good[1] && pos0 + DEC_KEYS <= sq.len;
-#pragma unroll
-      for (int z = 0; z < 2; ++z) {  // 16 keys of one page
-        const int pos = pos0 + 16 * z, pg = good[z] ? page[z] : 0;
-        const int r = pos - page_of(a.c, pos) * a.c.page_size;
-        const uint8_t* kp = kh + (static_cast<int64_t>(pg) * a.c.k_page16 << 4);
-        const uint8_t* vp = vh + (static_cast<int64_t>(pg) * a.c.v_page16 << 4);
-        if constexpr (STEP <= 16) {
-          kp += static_cast<int64_t>(r + my_row) * a.c.k_row;
-          vp += static_cast<int64_t>(r + my_row) * a.c.v_row;
-#pragma unroll
-          for (int i = 0; i < 16 / STEP; ++i) {
-            const int row = 16 * z + i * STEP + my_row;
-            const uint32_t dk = st + row * D + ((my_piece ^ C::swz_k(row)) << 4);
-            const uint32_t dv = st + C::CODES + row * D + ((my_piece ^ C::swz_v(row)) << 4);
-            if (full) {
-              cp_async16_full(dk, kp + static_cast<int64_t>(i * STEP) * a.c.k_row);
-              cp_async16_full(dv, vp + static_cast<int64_t>(i * STEP) * a.c.v_row);
-            } else {  // rows past the end or of a refused page hold anything: zeros instead
-              const bool in = good[z] && pos0 + row < sq.len;
-              cp_async16(dk, in ? kp + static_cast<int64_t>(i * STEP) * a.c.k_row : kh, in);
-              cp_async16(dv, in ? vp + static_cast<int64_t>(i * STEP) * a.c.v_row : vh, in);
-            }
-          }
-        } else if (my_row / 16 == z) {  // D = 16: 32 rows at once
-          const int64_t rr = r + (my_row & 15);
-          const bool in = good[z] && pos0 + my_row < sq.len;
-          cp_async16(st + my_row * D, in ? kp + rr * a.c.k_row : kh, in);
-          cp_async16(st + C::CODES + my_row * D, in ? vp + rr * a.c.v_row : vh, in);
+      const int page[2] = {next_page[0], next_page[1]}, r0 = row_in, pos0 = group_pos(it);
+      if (a.c.page_size < 128) {
+        pi += 128 >> a.c.page_shift;
+      } else {
+        row_in += 128;
+        if (row_in >= a.c.page_size) {
+          row_in -= a.c.page_size;
+          ++pi;
         }
-        if (lane / 16 == z) {
-          const int64_t rr = r + (lane & 15);
-          const bool in = good[z] && pos0 + lane < sq.len;
-          if (good[z]) {
-            cp_async4(sc, in ? ksh + static_cast<int64_t>(pg) * a.c.ks_page + rr * a.c.ks_row : ksh, in);
-            cp_async4(sc + DEC_KEYS * 4, in ? vsh + static_cast<int64_t>(pg) * a.c.vs_page + rr * a.c.vs_row : vsh, in);
-          } else {  // a refused page: queries that see its keys get NaN
-            asm volatile("st.shared.b32 [%0], %1;" ::"r"(sc), "r"(0x7fc00000u) : "memory");
-            asm volatile("st.shared.b32 [%0], %1;" ::"r"(sc + DEC_KEYS * 4), "r"(0u) : "memory");
+      }
+      fetch_pages(it + 1);
+      const uint32_t st = ring + (it % DEC_STAGES) * C::STAGE;
+      const uint32_t sc = st + 2 * C::CODES + lane * 4;
+      const bool good[2] = {static_cast<unsigned>(page[0]) < static_cast<unsigned>(a.c.num_pages),
+                            static_cast<unsigned>(page[1]) < static_cast<unsigned>(a.c.num_pages)};
+      if (good[0] && good[1] && pos0 + DEC_KEYS <= sq.len && STEP <= 16) {
+        const uint8_t* kp = kh + (static_cast<int64_t>(page[0]) * a.c.k_page16 << 4) + static_cast<int64_t>(r0 + my_row) * a.c.k_row;
+        const uint8_t* vp = vh + (static_cast<int64_t>(page[0]) * a.c.v_page16 << 4) + static_cast<int64_t>(r0 + my_row) * a.c.v_row;
+#pragma unroll
+        for (int i = 0; i < C::PIECES; ++i) {
+          if (i == C::PIECES / 2 && two) {
+            kp = kh + (static_cast<int64_t>(page[1]) * a.c.k_page16 << 4) + static_cast<int64_t>(my_row) * a.c.k_row;
+            vp = vh + (static_cast<int64_t>(page[1]) * a.c.v_page16 << 4) + static_cast<int64_t>(my_row) * a.c.v_row;
           }
+          // Row i STEP + my_row; its swizzle differs from my_row's by that of i STEP.
+          cp_async16_full(st + i * STEP * D + (to_k ^ (C::swz_k(i * STEP) << 4)), kp);
+          cp_async16_full(st + C::CODES + i * STEP * D + (to_v ^ (C::swz_v(i * STEP) << 4)), vp);
+          kp += step_k;
+          vp += step_v;
+        }
+        const int pg = lane < 16 ? page[0] : page[1], r = two ? lane & 15 : r0 + lane;
+        cp_async4(sc, ksh + static_cast<int64_t>(pg) * a.c.ks_page + static_cast<int64_t>(r) * a.c.ks_row, true);
+        cp_async4(sc + DEC_KEYS * 4, vsh + static_cast<int64_t>(pg) * a.c.vs_page + static_cast<int64_t>(r) * a.c.vs_row, true);
+      } else {
+        // Rows past the end hold anything: zeros instead. A refused page: zeros and NaN scales,
+        // queries that see its keys get NaN.
+        if (!good[0] || !good[1]) report(a.err, FA2_ERR_PAGE);
+        for (int i = 0; i < C::PIECES; ++i) {
+          const int row = i * STEP + my_row;
+          const bool ok = row < 16 ? good[0] : good[1], in = ok && pos0 + row < sq.len;
+          const int pg = in ? (row < 16 ? page[0] : page[1]) : 0, r = in ? (two ? row & 15 : r0 + row) : 0;
+          cp_async16(st + row * D + ((my_piece ^ C::swz_k(row)) << 4),
+                     kh + (static_cast<int64_t>(pg) * a.c.k_page16 << 4) + static_cast<int64_t>(r) * a.c.k_row, in);
+          cp_async16(st + C::CODES + row * D + ((my_piece ^ C::swz_v(row)) << 4),
+                     vh + (static_cast<int64_t>(pg) * a.c.v_page16 << 4) + static_cast<int64_t>(r) * a.c.v_row, in);
+        }
+        const bool ok = lane < 16 ? good[0] : good[1], in = ok && pos0 + lane < sq.len;
+        const int pg = in ? (lane < 16 ? page[0] : page[1]) : 0, r = in ? (two ? lane & 15 : r0 + lane) : 0;
+        if (ok) {
+          cp_async4(sc, ksh + static_cast<int64_t>(pg) * a.c.ks_page + static_cast<int64_t>(r) * a.c.ks_row, in);
+          cp_async4(sc + DEC_KEYS * 4, vsh + static_cast<int64_t>(pg) * a.c.vs_page + static_cast<int64_t>(r) * a.c.vs_row, in);
+        } else {
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(sc), "r"(0x7fc00000u) : "memory");
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(sc + DEC_KEYS * 4), "r"(0u) : "memory");
         }
       }
     }
