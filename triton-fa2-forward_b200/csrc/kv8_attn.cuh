@@ -24,20 +24,29 @@ struct AttnArgs {
   const int* lens;
   const int* cu_q;  // packed queries, else nullptr
   int* err;
-  float* o_part;    // split partials: O / l in fp32 ...
+  float* o_part;    // partial results: O / l in fp32 ...
   float* lse_part;  // ... and log2 of the row's sum
+  struct Cut* cuts;  // [workers]
   int64_t bt_stride;
   long long timeout;
   int pages_per_seq, batch, group, heads_kv, n_q, total_q, max_k;
+  uint32_t group_mul;  // rows to queries: n / group = hi(n * mul) >> shift
+  int group_shift;
   int causal, bottom_right;
-  int splits, split_keys;  // key ranges [s * split_keys, (s + 1) * split_keys)
-  int row_blocks, rows_pad;
+  int workers;  // CTAs that share the work
+  int block;    // rows of a block: 8, 16 or 256
   float qk_scale;
 };
 
 constexpr float RESCALE_TH = 8.0f;  // log2: the reference max moves when a row's max grows by more
 constexpr int P_SHIFT = 6;          // P' = p * sv * 2^(P_SHIFT - e), see above
 constexpr int EB_MIN = 8;           // smallest exponent field used for e (a multiplier stays finite)
+
+// n / group and n - group * (n / group) for 0 <= n < 2^31 (mul = 2^(31 + s) / group + 1 with group <= 2^s:
+// the product is too large by less than n 2^-(31 + s) < 1 / group).
+__device__ __forceinline__ int query_of(const AttnArgs& a, int row) {
+  return a.group == 1 ? row : static_cast<int>(__umulhi(static_cast<uint32_t>(row), a.group_mul) >> a.group_shift);
+}
 
 struct Seq {
   int n_q, q0, len, off;  // queries, first packed row, keys, causal offset
@@ -71,7 +80,7 @@ __device__ __forceinline__ Seq sequence(const AttnArgs& a, int b) {
 // Keys that the rows [row0, row0 + count) of a (sequence, kv head) see at most: [0, result).
 __device__ __forceinline__ int keys_end(const AttnArgs& a, const Seq& s, int row0, int count) {
   if (!a.causal) return s.len;
-  const int i = min((row0 + count - 1) / a.group, s.n_q - 1);
+  const int i = min(query_of(a, row0 + count - 1), s.n_q - 1);
   return max(0, min(s.len, i + s.off + 1));
 }
 
@@ -81,16 +90,182 @@ __device__ __forceinline__ int last_key(const AttnArgs& a, const Seq& s, int i) 
 }
 
 __device__ __forceinline__ const uint16_t* q_row(const AttnArgs& a, const Seq& s, int b, int h, int row) {
-  const int i = row / a.group, g = row - i * a.group;
+  const int i = query_of(a, row), g = row - i * a.group;
   const int64_t bb = a.cu_q != nullptr ? 0 : b;
   return a.q + bb * a.q_st[0] + static_cast<int64_t>(h * a.group + g) * a.q_st[1] + static_cast<int64_t>(s.q0 + i) * a.q_st[2];
 }
 
 __device__ __forceinline__ uint16_t* o_row(const AttnArgs& a, const Seq& s, int b, int h, int row) {
-  const int i = row / a.group, g = row - i * a.group;
+  const int i = query_of(a, row), g = row - i * a.group;
   const int64_t bb = a.cu_q != nullptr ? 0 : b;
   return a.o + bb * a.o_st[0] + static_cast<int64_t>(h * a.group + g) * a.o_st[1] + static_cast<int64_t>(s.q0 + i) * a.o_st[2];
 }
+
+// A row block that is cut for the first time by the start of worker w's share, written by that worker
+// for the merge kernel: its parts are those of the workers w - 1, w, w + 1, ...
+struct Cut {
+  int n_parts;  // 0: this share's start cuts no block, or not as the first
+  int b, h, row0;
+  int q0, n_q;     // of the sequence
+  int first_slot;  // of worker w - 1's part; worker v's is 2 v from w on
+  int unused;
+};
+
+// The work of a call, as one line of tiles: sequence by sequence, kv head by kv head, row block by
+// row block, 128 keys a tile. Each of W workers takes N / W of the line's N cost units (one more for the
+// first N % W), whatever the sequences' lengths: nobody waits for a longer sequence, and the lengths may live on the
+// device. A (sequence, head, block) that lies in one worker's share is written as the result; one
+// that is cut leaves a partial result for each share (a worker has at most two: where its share
+// begins and where it ends) and the merge kernel puts them together in the line's order.
+// A tile costs 1, or 2 where a CTA has two different 128-row tiles to do for it.
+struct Line {
+  // Tiles and tile cost of row block rb of sequence s, and the sum over a sequence's blocks.
+  __device__ static int blocks(const AttnArgs& a, const Seq& s) { return (s.n_q * a.group + a.block - 1) / a.block; }
+  __device__ static int tiles(const AttnArgs& a, const Seq& s, int rb) {
+    const int rows = s.n_q * a.group, row0 = rb * a.block;
+    return (keys_end(a, s, row0, min(a.block, rows - row0)) + 127) / 128;
+  }
+  __device__ static int tile_cost(const AttnArgs& a, const Seq& s, int rb) {
+    return a.block == 256 && s.n_q * a.group - rb * 256 > 128 ? 2 : 1;
+  }
+  __device__ static int head_cost(const AttnArgs& a, const Seq& s) {
+    int n = 0;
+    for (int rb = 0; rb < blocks(a, s); ++rb) n += tiles(a, s, rb) * tile_cost(a, s, rb);
+    return n;
+  }
+  // The workers that get something: with two cost units each at least, every share that begins or
+  // ends inside a block holds one of its tiles.
+  __device__ static int workers(const AttnArgs& a, int total) {
+    return min(a.workers, a.block == 256 ? (total + 1) / 2 : total);
+  }
+  // Where worker w's share starts, and the worker whose share holds position x.
+  __device__ static int start(int w, int workers, int total) {
+    const int q = total / workers;
+    return w * q + min(w, total - q * workers);
+  }
+  __device__ static int holder(int x, int workers, int total) {
+    const int q = total / workers, long_ones = total - q * workers;
+    return x < long_ones * (q + 1) ? x / (q + 1) : long_ones + (x - long_ones * (q + 1)) / q;
+  }
+};
+
+// Finds, with a warp, the length of the line, this worker's share of it and a sequence at or before
+// the share's start. Each lane adds up a run of sequences.
+struct Share {
+  int total, p0, p1;  // the line's length; this worker's share
+  int b, start_b;     // the first sequence of the run that holds p0, and where it starts
+};
+__device__ __forceinline__ Share find_share(const AttnArgs& a, int w) {
+  const int lane = static_cast<int>(threadIdx.x) & 31, per = (a.batch + 31) / 32;
+  const int b0 = min(a.batch, lane * per), b1 = min(a.batch, b0 + per);
+  int own = 0;
+#pragma unroll 1
+  for (int b = b0; b < b1; ++b) own += a.heads_kv * Line::head_cost(a, sequence(a, b));
+  int sum = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += v;
+  }
+  Share r;
+  r.total = __shfl_sync(0xffffffffu, sum, 31);
+  const int workers = Line::workers(a, r.total);
+  r.p0 = w < workers ? Line::start(w, workers, r.total) : 0;
+  r.p1 = w < workers ? Line::start(w + 1, workers, r.total) : 0;
+  const int before = sum - own;
+  const uint32_t at = __ballot_sync(0xffffffffu, before <= r.p0 && r.p0 < before + own);
+  const int from = at != 0 ? __ffs(at) - 1 : 0;
+  r.b = __shfl_sync(0xffffffffu, b0, from);
+  r.start_b = __shfl_sync(0xffffffffu, before, from);
+  return r;
+}
+
+// A row block and where it lies in the line.
+struct Block {
+  Seq sq;
+  int b, h, rb;
+  int at, tiles, cost;  // first position, tiles, cost of each
+  // The first tile at or behind position p. A share that begins or ends inside a tile: the tile
+  // belongs to the earlier worker.
+  __device__ int tile_of(int p) const { return p <= at ? 0 : min(tiles, (p - at + cost - 1) / cost); }
+};
+// The block that holds position p, walking on from sequence b, which starts at `start`.
+__device__ __forceinline__ void find_block(const AttnArgs& a, int p, int& b, int& start, Block& o) {
+  int hc;
+  while (true) {
+    o.sq = sequence(a, b);
+    hc = Line::head_cost(a, o.sq);
+    if (p < start + hc * a.heads_kv) break;
+    start += hc * a.heads_kv;
+    ++b;
+  }
+  o.b = b;
+  o.h = (p - start) / hc;
+  o.at = start + o.h * hc;
+  for (o.rb = 0;; ++o.rb) {
+    o.tiles = Line::tiles(a, o.sq, o.rb);
+    o.cost = Line::tile_cost(a, o.sq, o.rb);
+    if (p < o.at + o.tiles * o.cost) return;
+    o.at += o.tiles * o.cost;
+  }
+}
+
+// A piece of a worker's share: tiles of one row block.
+struct Piece {
+  Seq sq;
+  int b, h, rb;
+  int t0, tiles;  // the first tile and how many
+  int kend;       // keys that the block's rows see: [0, kend)
+  int slot;       // where a partial result goes, -1 for a whole one
+};
+// The pieces of a share in order; a warp walks them (uniformly) and also leaves the share's Cut.
+struct Pieces {
+  Share s;
+  int p, w;
+  __device__ void begin(const AttnArgs& a, int worker) {
+    s = find_share(a, worker);
+    p = s.p0;
+    w = worker;
+    if (s.p0 >= s.p1) a.cuts[w].n_parts = 0;
+  }
+  __device__ bool next(const AttnArgs& a, Piece& o) {
+    while (p < s.p1) {
+      Block k;
+      find_block(a, p, s.b, s.start_b, k);
+      o.sq = k.sq;
+      o.b = k.b;
+      o.h = k.h;
+      o.rb = k.rb;
+      o.t0 = k.tile_of(p);
+      o.tiles = k.tile_of(s.p1) - o.t0;
+      const int row0 = o.rb * a.block;
+      o.kend = keys_end(a, o.sq, row0, min(a.block, o.sq.n_q * a.group - row0));
+      if (p == s.p0) {
+        const int workers = Line::workers(a, s.total), before = w > 0 ? Line::start(w - 1, workers, s.total) : 0;
+        Cut c{};
+        if (o.tiles > 0 && o.t0 > 0 && k.tile_of(before) == 0) {
+          // (A tile is its start's holder's. Shares of two units and more between hold one each.)
+          c.n_parts = Line::holder(k.at + (k.tiles - 1) * k.cost, workers, s.total) - w + 2;
+          c.b = o.b;
+          c.h = o.h;
+          c.row0 = row0;
+          c.q0 = o.sq.q0;
+          c.n_q = o.sq.n_q;
+          c.first_slot = 2 * (w - 1) + (before >= k.at ? 0 : 1);
+        }
+        a.cuts[w] = c;
+      }
+      o.slot = o.tiles == k.tiles ? -1 : 2 * w + (p == s.p0 ? 0 : 1);
+      p = min(s.p1, k.at + k.tiles * k.cost);
+      if (o.tiles > 0) return true;
+    }
+    return false;
+  }
+};
+
+// A later kernel of the stream may start before this one ends (it waits for its results itself).
+__device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }  // -126 <= e <= 127
 

@@ -3,6 +3,7 @@
 #include "kv8_attn.cuh"
 #include "kv8_chunk.cuh"
 
+#include <algorithm>
 #include <cmath>
 
 namespace {
@@ -31,6 +32,7 @@ using namespace fa2kv;
 constexpr int DEC_WARPS = 4;
 constexpr int DEC_KEYS = 32;   // of a group
 constexpr int DEC_STAGES = 2;  // 12 warps an SM x one group on its way: 96 KB
+constexpr int DEC_CTAS = 3;    // an SM
 
 template <int D>
 struct Dec {
@@ -89,30 +91,19 @@ __device__ __forceinline__ float keys_sum(float x) {
 }
 
 // NT: 8-row tiles of the row block (1 or 2).
+// One worker's part of the keys of one (sequence, kv head): keys [k0, k1). `slot`: where a partial
+// result goes, -1 for a whole one.
 template <int D, bool BF16, int NT>
-__global__ void __launch_bounds__(DEC_WARPS * 32, 3) decode_kernel(const AttnArgs a) {
+__device__ __forceinline__ void decode_part(const AttnArgs& a, uint8_t* smem, const Seq& sq, int b, int h, int k0, int k1, int slot) {
   using C = Dec<D>;
   constexpr int ROWS = 8 * NT;
-  extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
-  // Row blocks of one key range run next to one another: they share its bytes in L2.
-  int x = static_cast<int>(blockIdx.x);
-  const int rb = x % a.row_blocks;
-  x /= a.row_blocks;
-  const int split = x % a.splits;
-  x /= a.splits;
-  const int h = x % a.heads_kv, b = x / a.heads_kv;
-  const Seq sq = sequence(a, b);
-  const int rows = sq.n_q * a.group, row0 = rb * ROWS;
-  if (row0 >= rows) return;
-  const int kend = keys_end(a, sq, row0, min(ROWS, rows - row0));
-  const int k0 = split * a.split_keys;
-  const int k1 = min(kend, k0 + a.split_keys);
-  if (k1 <= k0 && a.splits > 1) return;  // the merge kernel does not read this split
+  const int rows = sq.n_q * a.group;
+  constexpr int row0 = 0;
 
   const uint32_t ring = fa2::smem_u32(smem) + warp * C::RING;
-  const int n_groups = k1 > k0 ? (k1 - k0 + DEC_KEYS - 1) / DEC_KEYS : 0;
+  const int n_groups = (k1 - k0 + DEC_KEYS - 1) / DEC_KEYS;
   const int mine = n_groups > warp ? (n_groups - warp + DEC_WARPS - 1) / DEC_WARPS : 0;
   const int* bt = a.bt + b * a.bt_stride;
   // A lane copies piece lane % PIECES of the rows lane / PIECES + STEP * i of a group, and the scales
@@ -248,12 +239,12 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, 3) decode_kernel(const AttnArg
     for (int i = 0; i < 2; ++i) {
       const int r = 8 * t + 2 * c + i;
       row_sc[t][i] = q_scale[warp][r];
-      lim[t][i] = row0 + r < rows ? last_key(a, sq, (row0 + r) / a.group) : -1;
+      lim[t][i] = row0 + r < rows ? last_key(a, sq, query_of(a, row0 + r)) : -1;
       m[t][i] = -INFINITY;
       l[t][i] = 0.0f;
     }
   }
-  const int lim_first = last_key(a, sq, row0 / a.group);  // the smallest of the block's rows
+  const int lim_first = last_key(a, sq, query_of(a, row0));  // the smallest of the block's rows
 
   float o[NT][D / 16][4];
 #pragma unroll
@@ -466,7 +457,7 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, 3) decode_kernel(const AttnArg
   constexpr int PARTS = DEC_WARPS * 32 / ROWS;  // threads of a row
   const int r = static_cast<int>(threadIdx.x) / PARTS, part = static_cast<int>(threadIdx.x) % PARTS;
   const int row = row0 + r;
-  if (row >= rows) return;
+  if (row >= rows) return;  // (no barrier follows in here)
   float mx = -INFINITY;
 #pragma unroll
   for (int w = 0; w < DEC_WARPS; ++w) mx = fmaxf(mx, wm[w * 16 + r]);
@@ -479,7 +470,7 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, 3) decode_kernel(const AttnArg
     sum = f[w] == 0.0f ? sum : fmaf(f[w], lw, sum);
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  const int64_t slot = (static_cast<int64_t>(b * a.heads_kv + h) * a.splits + split) * a.rows_pad + row;
+  const int64_t part_row = static_cast<int64_t>(slot) * ROWS + row;
   constexpr int PER = D / PARTS > 0 ? (D / PARTS < 8 ? D / PARTS : 8) : 1;  // neighbouring columns at a time
   for (int d = part * PER; d < D; d += PARTS * PER) {
     float acc[PER] = {};
@@ -490,9 +481,9 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, 3) decode_kernel(const AttnArg
 #pragma unroll
       for (int j = 0; j < PER; ++j) acc[j] = fmaf(f[w], src[j], acc[j]);
     }
-    if (a.splits > 1) {
+    if (slot >= 0) {
 #pragma unroll
-      for (int j = 0; j < PER; ++j) a.o_part[slot * D + d + j] = acc[j] * inv;
+      for (int j = 0; j < PER; ++j) a.o_part[part_row * D + d + j] = acc[j] * inv;
     } else {
       uint16_t* dst = o_row(a, sq, b, h, row) + d;
       if constexpr (PER >= 2) {
@@ -505,96 +496,130 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, 3) decode_kernel(const AttnArg
       }
     }
   }
-  if (a.splits > 1 && part == 0) a.lse_part[slot] = sum == 0.0f ? -INFINITY : (mx == -INFINITY ? 0.0f : mx) + log2f(sum);
+  if (slot >= 0 && part == 0) a.lse_part[part_row] = sum == 0.0f ? -INFINITY : (mx == -INFINITY ? 0.0f : mx) + log2f(sum);
 }
 
-// ------------------------------------------------------------------ merge of the key ranges
-// One warp a row: o = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max) in split order.
+template <int D, bool BF16, int NT>
+__global__ void __launch_bounds__(DEC_WARPS * 32, DEC_CTAS) decode_kernel(const AttnArgs a) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  allow_next();
+  __shared__ Piece piece;
+  __shared__ int more;
+  Pieces pieces;
+  if (threadIdx.x < 32) pieces.begin(a, static_cast<int>(blockIdx.x));
+  while (true) {
+    if (threadIdx.x < 32) {  // warp 0 walks the share
+      Piece o{};
+      const bool m = pieces.next(a, o);
+      if (threadIdx.x == 0) {
+        piece = o;
+        more = m;
+      }
+    }
+    __syncthreads();
+    if (!more) break;
+    const Piece o = piece;
+    decode_part<D, BF16, NT>(a, smem, o.sq, o.b, o.h, o.t0 * 128, min(o.kend, (o.t0 + o.tiles) * 128), o.slot);
+    __syncthreads();  // the shared memory is free again
+  }
+}
+
+// ------------------------------------------------------------------ merge of the partial results
+// o = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max) over a cut block's parts, in the line's order, a
+// warp a row: CTA (x, y) has the rows [8 y, 8 y + 8) of the block that share x + 1 is the first to cut.
+// The last ZERO_CTAS write zeros for the blocks without a tile, which no worker has.
+constexpr int ZERO_CTAS = 16;
+constexpr int MERGE_ROWS = 8;
+
 template <int D, bool BF16>
-__global__ void __launch_bounds__(128) merge_kernel(const AttnArgs a, int block) {
+__global__ void __launch_bounds__(128) merge_kernel(const AttnArgs a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t x = static_cast<int64_t>(blockIdx.x) * 4 + warp;
-  const int row = static_cast<int>(x % a.rows_pad);
-  const int bh = static_cast<int>(x / a.rows_pad);
-  if (bh >= a.batch * a.heads_kv) return;
-  const int b = bh / a.heads_kv, h = bh - b * a.heads_kv;
-  const Seq sq = sequence(a, b);
-  const int rows = sq.n_q * a.group;
-  if (row >= rows) return;
-  const int row0 = row / block * block;
-  const int ns = (keys_end(a, sq, row0, min(block, rows - row0)) + a.split_keys - 1) / a.split_keys;
-  const float* lse = a.lse_part + static_cast<int64_t>(bh) * a.splits * a.rows_pad + row;
-  const float* op = a.o_part + (static_cast<int64_t>(bh) * a.splits * a.rows_pad + row) * D;
-  float mx = -INFINITY;
-  for (int s = lane; s < ns; s += 32) mx = fmaxf(mx, lse[static_cast<int64_t>(s) * a.rows_pad]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  const int row_first = static_cast<int>(blockIdx.y) * MERGE_ROWS;
+  const int w = static_cast<int>(blockIdx.x) + 1;
+  wait_for_previous();  // every thread: what follows this kernel must not overtake the one before it
+  if (w >= a.workers) {
+    for (int b = w - a.workers; b < a.batch; b += ZERO_CTAS) {
+      const Seq sq = sequence(a, b);
+      const int rows = sq.n_q * a.group;
+      for (int rb = 0; rb * a.block < rows; ++rb) {
+        if (Line::tiles(a, sq, rb) > 0) continue;
+        const int row0 = rb * a.block + row_first, n = min(min(MERGE_ROWS, a.block - row_first), rows - row0);
+        for (int i = threadIdx.x; i < n * a.heads_kv; i += 128) {
+          uint4* dst = reinterpret_cast<uint4*>(o_row(a, sq, b, i / n, row0 + i % n));
+#pragma unroll 1
+          for (int j = 0; j < D / 8; ++j) dst[j] = make_uint4(0, 0, 0, 0);
+        }
+      }
+    }
+    return;
+  }
+  const Cut cut = a.cuts[w];
+  Seq sq{};
+  sq.q0 = cut.q0;
+  const int rows = min(a.block, cut.n_q * a.group - cut.row0);
   constexpr int PER = D >= 32 ? D / 32 : 1;
   const bool on = lane * PER < D;
-  float acc[PER] = {}, sum = 0.0f;
-  for (int s0 = 0; s0 < ns; s0 += 32) {
-    float w = 0.0f;
-    if (s0 + lane < ns) {
-      const float v = lse[static_cast<int64_t>(s0 + lane) * a.rows_pad];
-      w = v == -INFINITY ? 0.0f : exp2f(v - (mx == -INFINITY ? 0.0f : mx));  // a NaN stays one
-    }
-    const int n = min(32, ns - s0);
-#pragma unroll 4
-    for (int s = 0; s < n; ++s) {
-      const float f = __shfl_sync(0xffffffffu, w, s);
-      if (on && f != 0.0f) {
-        const float* src = op + static_cast<int64_t>(s0 + s) * a.rows_pad * D + lane * PER;
+  auto part = [&](int i, int r) -> int64_t {  // its row
+    return static_cast<int64_t>(i == 0 ? cut.first_slot : 2 * (w - 1 + i)) * a.block + r;
+  };
+  if (cut.n_parts == 0) return;
+  for (int r = row_first + warp; r < min(rows, row_first + MERGE_ROWS); r += 4) {
+    float mx = -INFINITY;
+    for (int i = lane; i < cut.n_parts; i += 32) mx = fmaxf(mx, a.lse_part[part(i, r)]);
 #pragma unroll
-        for (int i = 0; i < PER; ++i) acc[i] = fmaf(f, src[i], acc[i]);
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    float acc[PER] = {}, sum = 0.0f;
+    for (int i0 = 0; i0 < cut.n_parts; i0 += 32) {
+      const float v = i0 + lane < cut.n_parts ? a.lse_part[part(i0 + lane, r)] : -INFINITY;
+      const float f = v == -INFINITY ? 0.0f : exp2f(v - (mx == -INFINITY ? 0.0f : mx));  // a NaN stays one
+      const int n = min(32, cut.n_parts - i0);
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const float fi = __shfl_sync(0xffffffffu, f, i);
+        if (on && fi != 0.0f) {
+          const float* src = a.o_part + part(i0 + i, r) * D + lane * PER;
+#pragma unroll
+          for (int j = 0; j < PER; ++j) acc[j] = fmaf(fi, src[j], acc[j]);
+        }
+        sum += fi;
       }
-      sum += f;
+    }
+    if (on) {
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      uint16_t* dst = o_row(a, sq, cut.b, cut.h, cut.row0 + r) + lane * PER;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) dst[j] = x1_of_float<BF16>(acc[j] * inv);
     }
   }
-  if (!on) return;
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  uint16_t* dst = o_row(a, sq, b, h, row) + lane * PER;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) dst[i] = x1_of_float<BF16>(acc[i] * inv);
 }
 
 // ------------------------------------------------------------------------------------ host
 struct Plan {
   int block = 8;  // rows of a block: 8 or 16 (decode_kernel), 256 (chunk_kernel)
-  int row_blocks = 1, rows_pad = 16, splits = 1, split_keys = 0;
-  int64_t lse_floats = 0, bytes = 0;
+  int workers = 1;
+  int64_t cut_bytes = 0, lse_floats = 0, bytes = 0;
 };
 
 constexpr int MAX_SPLITS = 256;
 
-// The kernel and the key ranges of a call, from its sizes alone.
+// The kernel, the workers and the workspace of a call, from its sizes alone.
 Plan plan(const Fa2Kv8AttnParams* p) {
   Plan r;
   const int64_t rows = static_cast<int64_t>(p->seqlen_q) * (p->heads_q / p->cache.heads_kv);
   r.block = rows <= 8 ? 8 : rows <= 16 ? 16 : 256;
-  const bool chunk = r.block == 256;
-  r.row_blocks = static_cast<int>((rows + r.block - 1) / r.block);
-  r.rows_pad = r.row_blocks * r.block;
-  int64_t units = static_cast<int64_t>(p->batch) * p->cache.heads_kv * r.row_blocks;
-  if (units < 1) units = 1;
-  // Few rows: one wave of three CTAs on each of 148 SMs, at least one 32-key group for each of a
-  // CTA's warps. Many rows: one wave of one CTA an SM, at least four 128-key tiles each.
-  const int unit_keys = 128;  // one tile, or a group for each warp
-  int64_t s = p->num_splits > 0 ? p->num_splits : (chunk ? 148 : 148 * 3) / units;
-  const int64_t least = p->num_splits > 0 ? unit_keys : chunk ? 512 : 128;
-  const int64_t most = (p->max_seqlen_k + least - 1) / least;
-  if (s > most) s = most;
-  if (s > MAX_SPLITS) s = MAX_SPLITS;
-  if (s < 1) s = 1;
-  const int64_t per = (p->max_seqlen_k + s - 1) / s;
-  const int64_t keys = (per + unit_keys - 1) / unit_keys * unit_keys;
-  r.split_keys = static_cast<int>(keys < unit_keys ? unit_keys : keys > (1ll << 30) ? (1ll << 30) : keys);
-  r.splits = static_cast<int>((static_cast<int64_t>(p->max_seqlen_k) + r.split_keys - 1) / r.split_keys);
-  if (r.splits < 1) r.splits = 1;
-  if (r.splits > 1) {
-    const int64_t slots = static_cast<int64_t>(p->batch) * p->cache.heads_kv * r.splits * r.rows_pad;
-    r.lse_floats = (slots + 3) / 4 * 4;
-    r.bytes = 4 * (r.lse_floats + slots * p->cache.head_dim);
-  }
+  const int64_t units = static_cast<int64_t>(p->batch) * p->cache.heads_kv * std::max<int64_t>(1, (rows + r.block - 1) / r.block);
+  // One wave: DEC_CTAS CTAs, or one of the 256-row kernel, on each of 148 SMs.
+  const int64_t most = r.block == 256 ? 148 : 148 * DEC_CTAS;
+  const int64_t tiles = units * ((static_cast<int64_t>(p->max_seqlen_k) + 127) / 128);
+  int64_t w = p->num_splits > 0 ? units * p->num_splits : most;
+  if (w > most) w = most;
+  if (w > tiles) w = tiles;
+  r.workers = static_cast<int>(w < 1 ? 1 : w);
+  // A Cut and two partial results a worker.
+  const int64_t slots = 2ll * r.workers * r.block;
+  r.lse_floats = (slots + 3) / 4 * 4;
+  r.cut_bytes = static_cast<int64_t>(sizeof(Cut)) * r.workers;
+  r.bytes = r.cut_bytes + 4 * (r.lse_floats + slots * p->cache.head_dim);
   return r;
 }
 
@@ -617,14 +642,12 @@ int check_core(const Fa2Kv8AttnParams* p) {
   for (int i = 0; i < 3; ++i) {
     if (n[i] > 1 && ((p->q_stride[i] | p->o_stride[i]) & 7) != 0) return FA2_ERR_LAYOUT;
   }
-  // Row numbers and the grid stay in 31 bits.
+  // Row numbers, the line of tiles (two cost units each) and the grids stay in 31 bits.
   const int64_t rows = static_cast<int64_t>(p->seqlen_q) * (p->heads_q / p->cache.heads_kv);
-  if (rows > (1ll << 30)) return FA2_ERR_SHAPE;
-  if (static_cast<int64_t>(p->batch) * p->cache.heads_kv > (1ll << 26)) return FA2_ERR_SHAPE;
-  const Plan r = plan(p);
-  if (static_cast<int64_t>(p->batch) * p->cache.heads_kv * r.splits > (1ll << 32) / (r.rows_pad > 0 ? r.rows_pad : 1)) {
-    return FA2_ERR_SHAPE;
-  }
+  if (rows > (1ll << 30) || static_cast<int64_t>(p->batch) * p->cache.heads_kv > (1ll << 26)) return FA2_ERR_SHAPE;
+  const int64_t units = static_cast<int64_t>(p->batch) * p->cache.heads_kv * ((rows + 255) / 256);
+  const int64_t tiles = (static_cast<int64_t>(p->max_seqlen_k) + 127) / 128;
+  if (units > (1ll << 26) || units * tiles > (1ll << 29)) return FA2_ERR_SHAPE;
   return FA2_OK;
 }
 
@@ -637,15 +660,31 @@ bool allow_smem(K kernel, int bytes, int dev, std::atomic<bool> (&done)[MAX_DEVI
   return true;
 }
 
+// Launches the merge behind the kernel that was just launched. It may start early: it works out where
+// the parts lie, then waits for them.
 template <int D, bool BF16>
-int launch(const AttnArgs& a, int block, cudaStream_t s, int dev) {
+int launch_merge(const AttnArgs& a, cudaStream_t s) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.workers - 1 + ZERO_CTAS), (a.block + MERGE_ROWS - 1) / MERGE_ROWS);
+  cfg.blockDim = dim3(128);
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, merge_kernel<D, BF16>, a) == cudaSuccess ? FA2_OK : FA2_ERR_LAUNCH;
+}
+
+template <int D, bool BF16>
+int launch(const AttnArgs& a, cudaStream_t s, int dev) {
   static std::atomic<bool> done[3][MAX_DEVICES];
-  const unsigned ctas = static_cast<unsigned>(static_cast<int64_t>(a.batch) * a.heads_kv * a.splits * a.row_blocks);
-  if (block == 256) {
+  const unsigned ctas = static_cast<unsigned>(a.workers);
+  if (a.block == 256) {
     auto kernel = chunk_kernel<D, BF16>;
     if (!allow_smem(kernel, Ch<D, BF16>::SMEM, dev, done[2])) return FA2_ERR_LAUNCH;
     kernel<<<ctas, CH_THREADS, Ch<D, BF16>::SMEM, s>>>(a);
-  } else if (block == 16) {
+  } else if (a.block == 16) {
     auto kernel = decode_kernel<D, BF16, 2>;
     if (!allow_smem(kernel, Dec<D>::SMEM, dev, done[1])) return FA2_ERR_LAUNCH;
     kernel<<<ctas, DEC_WARPS * 32, Dec<D>::SMEM, s>>>(a);
@@ -655,10 +694,7 @@ int launch(const AttnArgs& a, int block, cudaStream_t s, int dev) {
     kernel<<<ctas, DEC_WARPS * 32, Dec<D>::SMEM, s>>>(a);
   }
   const int rc = launch_status();
-  if (rc != FA2_OK || a.splits <= 1) return rc;
-  const int64_t rows = static_cast<int64_t>(a.batch) * a.heads_kv * a.rows_pad;
-  merge_kernel<D, BF16><<<static_cast<unsigned>((rows + 3) / 4), 128, 0, s>>>(a, block);
-  return launch_status();
+  return rc != FA2_OK ? rc : launch_merge<D, BF16>(a, s);
 }
 
 }  // namespace
@@ -703,26 +739,31 @@ int fa2_kv8_attn_sm100(const Fa2Kv8AttnParams* p, void* stream) {
   a.pages_per_seq = p->pages_per_seq;
   a.batch = p->batch;
   a.group = p->heads_q / p->cache.heads_kv;
+  if (a.group > 1) {
+    int log = 1;
+    while ((1ll << log) < a.group) ++log;
+    a.group_mul = static_cast<uint32_t>((1ull << (31 + log)) / static_cast<uint64_t>(a.group) + 1);
+    a.group_shift = log - 1;
+  }
   a.heads_kv = p->cache.heads_kv;
   a.n_q = p->seqlen_q;
   a.total_q = p->total_q;
   a.max_k = p->max_seqlen_k;
   a.causal = p->causal;
   a.bottom_right = p->causal && p->causal_align == FA2_CAUSAL_BOTTOM_RIGHT;
-  a.splits = r.splits;
-  a.split_keys = r.split_keys;
-  a.row_blocks = r.row_blocks;
-  a.rows_pad = r.rows_pad;
+  a.workers = r.workers;
+  a.block = r.block;
   a.qk_scale = p->qk_scale;
-  a.lse_part = static_cast<float*>(p->workspace);
-  a.o_part = r.splits > 1 ? a.lse_part + r.lse_floats : nullptr;
+  a.cuts = static_cast<Cut*>(p->workspace);
+  a.lse_part = reinterpret_cast<float*>(static_cast<uint8_t*>(p->workspace) + r.cut_bytes);
+  a.o_part = a.lse_part + r.lse_floats;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf = p->dtype == FA2_DTYPE_BF16;
   switch (p->cache.head_dim) {
-    case 16: return bf ? launch<16, true>(a, r.block, s, dev) : launch<16, false>(a, r.block, s, dev);
-    case 32: return bf ? launch<32, true>(a, r.block, s, dev) : launch<32, false>(a, r.block, s, dev);
-    case 64: return bf ? launch<64, true>(a, r.block, s, dev) : launch<64, false>(a, r.block, s, dev);
-    default: return bf ? launch<128, true>(a, r.block, s, dev) : launch<128, false>(a, r.block, s, dev);
+    case 16: return bf ? launch<16, true>(a, s, dev) : launch<16, false>(a, s, dev);
+    case 32: return bf ? launch<32, true>(a, s, dev) : launch<32, false>(a, s, dev);
+    case 64: return bf ? launch<64, true>(a, s, dev) : launch<64, false>(a, s, dev);
+    default: return bf ? launch<128, true>(a, s, dev) : launch<128, false>(a, s, dev);
   }
 }
 
