@@ -112,8 +112,8 @@ struct Cut {
 };
 
 // The work of a call, as one line of tiles: sequence by sequence, kv head by kv head, row block by
-// row block, 128 keys a tile. Each of W workers takes N / W of the line's N cost units (one more for the
-// first N % W), whatever the sequences' lengths: nobody waits for a longer sequence, and the lengths may live on the
+// row block, 128 keys a tile. Worker w of W takes [w N / W, (w + 1) N / W) of the line's N cost units,
+// whatever the sequences' lengths: nobody waits for a longer sequence, and the lengths may live on the
 // device. A (sequence, head, block) that lies in one worker's share is written as the result; one
 // that is cut leaves a partial result for each share (a worker has at most two: where its share
 // begins and where it ends) and the merge kernel puts them together in the line's order.
@@ -139,13 +139,15 @@ struct Line {
     return min(a.workers, a.block == 256 ? (total + 1) / 2 : total);
   }
   // Where worker w's share starts, and the worker whose share holds position x.
-  __device__ static int start(int w, int workers, int total) {
-    const int q = total / workers;
-    return w * q + min(w, total - q * workers);
+  __device__ static int start(int w, int workers, int total) {  // w total / workers, in 32 bits
+    const uint32_t q = static_cast<uint32_t>(total) / static_cast<uint32_t>(workers), r = total - q * workers;
+    return static_cast<int>(w * q + w * r / static_cast<uint32_t>(workers));  // (w r < workers^2)
   }
   __device__ static int holder(int x, int workers, int total) {
-    const int q = total / workers, long_ones = total - q * workers;
-    return x < long_ones * (q + 1) ? x / (q + 1) : long_ones + (x - long_ones * (q + 1)) / q;
+    int w = min(workers - 1, static_cast<int>((x + 0.5f) * workers / total));  // off by one at most
+    while (w > 0 && start(w, workers, total) > x) --w;
+    while (w + 1 < workers && start(w + 1, workers, total) <= x) ++w;
+    return w;
   }
 };
 

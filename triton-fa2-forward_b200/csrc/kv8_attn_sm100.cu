@@ -32,7 +32,8 @@ using namespace fa2kv;
 constexpr int DEC_WARPS = 4;
 constexpr int DEC_KEYS = 32;   // of a group
 constexpr int DEC_STAGES = 2;  // 12 warps an SM x one group on its way: 96 KB
-constexpr int DEC_CTAS = 3;    // an SM
+constexpr int DEC_CTAS = 3;    // an SM at most
+constexpr int DEC_SHARES = 2;  // CTAs an SM that the work is shared among
 
 template <int D>
 struct Dec {
@@ -97,7 +98,7 @@ template <int D, bool BF16, int NT>
 __device__ __forceinline__ void decode_part(const AttnArgs& a, uint8_t* smem, const Seq& sq, int b, int h, int k0, int k1, int slot) {
   using C = Dec<D>;
   constexpr int ROWS = 8 * NT;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
   const int rows = sq.n_q * a.group;
   constexpr int row0 = 0;
@@ -501,7 +502,7 @@ __device__ __forceinline__ void decode_part(const AttnArgs& a, uint8_t* smem, co
 
 template <int D, bool BF16, int NT>
 __global__ void __launch_bounds__(DEC_WARPS * 32, DEC_CTAS) decode_kernel(const AttnArgs a) {
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ __align__(128) uint8_t smem[];  // (rows of codes start on their banks)
   allow_next();
   __shared__ Piece piece;
   __shared__ int more;
@@ -518,7 +519,18 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DEC_CTAS) decode_kernel(const 
     }
     __syncthreads();
     if (!more) break;
-    const Piece o = piece;
+    // (Broadcasts: what follows from these is then kept in uniform registers.)
+    Piece o;
+    o.sq.n_q = __shfl_sync(0xffffffffu, piece.sq.n_q, 0);
+    o.sq.q0 = __shfl_sync(0xffffffffu, piece.sq.q0, 0);
+    o.sq.len = __shfl_sync(0xffffffffu, piece.sq.len, 0);
+    o.sq.off = __shfl_sync(0xffffffffu, piece.sq.off, 0);
+    o.b = __shfl_sync(0xffffffffu, piece.b, 0);
+    o.h = __shfl_sync(0xffffffffu, piece.h, 0);
+    o.t0 = __shfl_sync(0xffffffffu, piece.t0, 0);
+    o.tiles = __shfl_sync(0xffffffffu, piece.tiles, 0);
+    o.kend = __shfl_sync(0xffffffffu, piece.kend, 0);
+    o.slot = __shfl_sync(0xffffffffu, piece.slot, 0);
     decode_part<D, BF16, NT>(a, smem, o.sq, o.b, o.h, o.t0 * 128, min(o.kend, (o.t0 + o.tiles) * 128), o.slot);
     __syncthreads();  // the shared memory is free again
   }
@@ -608,11 +620,13 @@ Plan plan(const Fa2Kv8AttnParams* p) {
   const int64_t rows = static_cast<int64_t>(p->seqlen_q) * (p->heads_q / p->cache.heads_kv);
   r.block = rows <= 8 ? 8 : rows <= 16 ? 16 : 256;
   const int64_t units = static_cast<int64_t>(p->batch) * p->cache.heads_kv * std::max<int64_t>(1, (rows + r.block - 1) / r.block);
-  // One wave: DEC_CTAS CTAs, or one of the 256-row kernel, on each of 148 SMs.
-  const int64_t most = r.block == 256 ? 148 : 148 * DEC_CTAS;
+  // One wave: DEC_SHARES CTAs, or one of the 256-row kernel, on each of 148 SMs; with fewer (sequence,
+  // head, block)s than that a multiple of their number, so that equal ones are cut alike.
+  const int64_t most = r.block == 256 ? 148 : 148 * DEC_SHARES;
   const int64_t tiles = units * ((static_cast<int64_t>(p->max_seqlen_k) + 127) / 128);
-  int64_t w = p->num_splits > 0 ? units * p->num_splits : most;
-  if (w > most) w = most;
+  int64_t w = p->num_splits > 0 ? units * p->num_splits : units < most && r.block < 256 ? most / units * units : most;
+  if (w > most && p->num_splits <= 0) w = most;
+  if (w > 148 * 16) w = 148 * 16;
   if (w > tiles) w = tiles;
   r.workers = static_cast<int>(w < 1 ? 1 : w);
   // A Cut and two partial results a worker.
