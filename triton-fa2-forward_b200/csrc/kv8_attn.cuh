@@ -30,8 +30,7 @@ struct AttnArgs {
   int64_t bt_stride;
   long long timeout;
   int pages_per_seq, batch, group, heads_kv, n_q, total_q, max_k;
-  uint32_t group_mul;  // rows to queries: n / group = hi(n * mul) >> shift
-  int group_shift;
+  Divisor by_group;  // rows to queries
   int causal, bottom_right;
   int workers;  // CTAs that share the work
   int block;    // rows of a block: 8, 16 or 256
@@ -42,11 +41,7 @@ constexpr float RESCALE_TH = 8.0f;  // log2: the reference max moves when a row'
 constexpr int P_SHIFT = 6;          // P' = p * sv * 2^(P_SHIFT - e), see above
 constexpr int EB_MIN = 8;           // smallest exponent field used for e (a multiplier stays finite)
 
-// n / group and n - group * (n / group) for 0 <= n < 2^31 (mul = 2^(31 + s) / group + 1 with group <= 2^s:
-// the product is too large by less than n 2^-(31 + s) < 1 / group).
-__device__ __forceinline__ int query_of(const AttnArgs& a, int row) {
-  return a.group == 1 ? row : static_cast<int>(__umulhi(static_cast<uint32_t>(row), a.group_mul) >> a.group_shift);
-}
+__device__ __forceinline__ int query_of(const AttnArgs& a, int row) { return divide(a.by_group, row); }
 
 struct Seq {
   int n_q, q0, len, off;  // queries, first packed row, keys, causal offset

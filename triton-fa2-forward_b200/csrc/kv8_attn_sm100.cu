@@ -753,12 +753,7 @@ int fa2_kv8_attn_sm100(const Fa2Kv8AttnParams* p, void* stream) {
   a.pages_per_seq = p->pages_per_seq;
   a.batch = p->batch;
   a.group = p->heads_q / p->cache.heads_kv;
-  if (a.group > 1) {
-    int log = 1;
-    while ((1ll << log) < a.group) ++log;
-    a.group_mul = static_cast<uint32_t>((1ull << (31 + log)) / static_cast<uint64_t>(a.group) + 1);
-    a.group_shift = log - 1;
-  }
+  a.by_group = divisor(a.group);
   a.heads_kv = p->cache.heads_kv;
   a.n_q = p->seqlen_q;
   a.total_q = p->total_q;

@@ -23,11 +23,13 @@ struct RowArgs {
   int* err;
   int64_t bt_stride;
   int pages_per_seq, batch, n;  // n: tokens of a sequence, or all packed rows
-  int64_t rows;                 // tokens * heads
+  int rows;                     // tokens * heads
+  Divisor by_heads, by_n;
+  bool wide;  // an input stride needs more than 32 bits
 };
 
 // Where a token lives: its page and row, or false where it is not to be touched.
-__device__ __forceinline__ bool find_row(const RowArgs& a, int b, int pos, int64_t& page, int& row) {
+__device__ __forceinline__ bool find_row(const RowArgs& a, int b, int pos, int& page, int& row) {
   const int pi = page_of(a.c, pos);
   if (pi >= a.pages_per_seq) {
     report(a.err, FA2_ERR_SHAPE);
@@ -43,57 +45,107 @@ __device__ __forceinline__ bool find_row(const RowArgs& a, int b, int pos, int64
   return true;
 }
 
-// Token t and head h of a block's thread. 32-bit arithmetic: the host bounds rows * L below 2^40
-// and the tokens below 2^31.
-__device__ __forceinline__ void token_head(const RowArgs& a, int64_t row, int& t, int& h) {
-  if (a.rows <= 0xffffffffll) {
-    const uint32_t q = static_cast<uint32_t>(row) / static_cast<uint32_t>(a.c.heads_kv);
-    t = static_cast<int>(q);
-    h = static_cast<int>(static_cast<uint32_t>(row) - q * a.c.heads_kv);
-  } else {
-    const int64_t q = row / a.c.heads_kv;
-    t = static_cast<int>(q);
-    h = static_cast<int>(row - q * a.c.heads_kv);
-  }
+__device__ __forceinline__ void token_head(const RowArgs& a, int row, int& t, int& h) {
+  t = divide(a.by_heads, row);
+  h = row - t * a.c.heads_kv;
 }
 
-template <bool BF16, bool VEC>
-__device__ __forceinline__ void load16(const uint16_t* x, int64_t d_stride, float (&f)[16]) {
+// Bytes (codes) or entries (scales) from a tensor's start to a row: widening 32-bit products.
+__device__ __forceinline__ int64_t codes_at(const Cache& c, bool v, int page, int row, int h) {
+  return (static_cast<int64_t>(page) * (v ? c.v_page16 : c.k_page16) << 4) + static_cast<int64_t>(row) * (v ? c.v_row : c.k_row) +
+         static_cast<int64_t>(h) * (v ? c.v_head : c.k_head);
+}
+__device__ __forceinline__ int64_t scale_at(const Cache& c, bool v, int page, int row, int h) {
+  return static_cast<int64_t>(page) * (v ? c.vs_page : c.ks_page) + static_cast<int64_t>(row) * (v ? c.vs_row : c.ks_row) +
+         static_cast<int64_t>(h) * (v ? c.vs_head : c.ks_head);
+}
+
+// An input row. Strides fit 32 bits unless the host says otherwise.
+__device__ __forceinline__ const uint16_t* row_at(const RowArgs& a, int z, int b, int h, int n) {
+  if (a.wide) return a.x[z] + b * a.st[z][0] + h * a.st[z][1] + n * a.st[z][2];
+  return a.x[z] + static_cast<int64_t>(b) * static_cast<int>(a.st[z][0]) + static_cast<int64_t>(h) * static_cast<int>(a.st[z][1]) +
+         static_cast<int64_t>(n) * static_cast<int>(a.st[z][2]);
+}
+
+// 16 values of a row as they are in memory, and as floats.
+template <bool VEC>
+__device__ __forceinline__ void load16(const uint16_t* x, int64_t d_stride, uint32_t (&w)[8]) {
   if constexpr (VEC) {
-    const uint4 w0 = *reinterpret_cast<const uint4*>(x), w1 = *reinterpret_cast<const uint4*>(x + 8);
-    const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+    const uint4 w0 = __ldcs(reinterpret_cast<const uint4*>(x)), w1 = __ldcs(reinterpret_cast<const uint4*>(x) + 1);
+    w[0] = w0.x;
+    w[1] = w0.y;
+    w[2] = w0.z;
+    w[3] = w0.w;
+    w[4] = w1.x;
+    w[5] = w1.y;
+    w[6] = w1.z;
+    w[7] = w1.w;
+  } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float2 v = float2_of_x2<BF16>(w[i]);
-      f[2 * i] = v.x;
-      f[2 * i + 1] = v.y;
+      w[i] = static_cast<uint32_t>(x[2 * i * d_stride]) | (static_cast<uint32_t>(x[(2 * i + 1) * d_stride]) << 16);
     }
-  } else {
+  }
+}
+template <bool BF16>
+__device__ __forceinline__ void floats16(const uint32_t (&w)[8], float (&f)[16]) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) f[i] = float_of_16<BF16>(x[i * d_stride]);
+  for (int i = 0; i < 8; ++i) {
+    const float2 v = float2_of_x2<BF16>(w[i]);
+    f[2 * i] = v.x;
+    f[2 * i + 1] = v.y;
   }
 }
 
-// The row's scale from its lanes' values; NaN where a value is not finite.
-template <int L>
-__device__ __forceinline__ float row_scale(const float (&f)[16]) {
-  uint32_t m = 0;  // magnitudes compare as integers, NaN above infinity: nothing is lost in the max
+// The row's scale from its lanes' values; NaN where a value is not finite. The magnitudes' largest is
+// taken two at a time in the type itself (exact; a NaN wins).
+template <int L, bool BF16>
+__device__ __forceinline__ float row_scale(const uint32_t (&w)[8]) {
+  auto larger = [](uint32_t x, uint32_t y) -> uint32_t {
+    uint32_t r;
+    if constexpr (BF16) {
+      asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+    } else {
+      asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+    }
+    return r;
+  };
+  uint32_t m = w[0] & 0x7fff7fffu;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
+  for (int i = 1; i < 8; ++i) m = larger(m, w[i] & 0x7fff7fffu);
+  m = larger(m, __byte_perm(m, m, 0x1032));
 #pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-  return m < 0x7f800000u ? __uint_as_float(m) / E4M3_MAX : __uint_as_float(0x7fc00000u);
+  for (int o = L / 2; o > 0; o >>= 1) m = larger(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float top = float2_of_x2<BF16>(m).x;
+  return top < INFINITY ? top / E4M3_MAX : __uint_as_float(0x7fc00000u);
 }
 
+// x / scale, correctly rounded, by Markstein's theorem (1990): with r the rounded reciprocal of scale
+// and q = x r, q + r (x - q scale) in fused multiply-adds is the rounded quotient. Three instructions
+// where the division takes about ten; for scales where r or the remainder could leave the normal
+// range (a largest value below 2^-71) the division itself.
 __device__ __forceinline__ uint4 codes16(const float (&f)[16], float scale) {
   const bool some = scale > 0.0f;  // false for a zero row and for a NaN scale: codes 0
+  const bool plain = scale > 0x1p-80f && scale < 0x1p120f;
+  const float r = plain ? 1.0f / scale : 0.0f;
+  float q[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float q0 = f[i] * r;
+    q[i] = fmaf(fmaf(-q0, scale, f[i]), r, q0);
+  }
+  if (some && !plain) {
+#pragma unroll 1
+    for (int i = 0; i < 16; ++i) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) q[j] = j == i ? f[j] / scale : q[j];
+    }
+  }
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float q[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) q[j] = some ? f[4 * i + j] / scale : 0.0f;
-    w[i] = static_cast<uint32_t>(e4m3x2(q[0], q[1])) | (static_cast<uint32_t>(e4m3x2(q[2], q[3])) << 16);
+    w[i] = some ? static_cast<uint32_t>(e4m3x2(q[4 * i], q[4 * i + 1])) | (static_cast<uint32_t>(e4m3x2(q[4 * i + 2], q[4 * i + 3])) << 16)
+                : 0u;
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
@@ -101,15 +153,22 @@ __device__ __forceinline__ uint4 codes16(const float (&f)[16], float scale) {
 template <int D, bool BF16, bool VEC>
 __global__ void __launch_bounds__(128) append_kernel(const RowArgs a) {
   constexpr int L = D / 16;
-  const int64_t idx0 = static_cast<int64_t>(blockIdx.x) * 128;
-  const int64_t row_id = (idx0 + threadIdx.x) / L;
-  const int part = threadIdx.x % L;
+  constexpr int ROWS = 128 / L;  // of a block
+  const int first = static_cast<int>(blockIdx.x) * ROWS;
+  const int part = threadIdx.x % L, row_id = first + static_cast<int>(threadIdx.x) / L;
   bool on = row_id < a.rows;
   int t = 0, h = 0, b, i, n_new;
   token_head(a, on ? row_id : a.rows - 1, t, h);
+  // The rows are asked for before the way to their pages is walked.
+  uint32_t raw[2][8];
+  const int tb = a.cu != nullptr ? 0 : divide(a.by_n, t), tn = a.cu != nullptr ? t : t - tb * a.n;
+#pragma unroll
+  for (int z = 0; z < 2; ++z) {
+    load16<VEC>(row_at(a, z, tb, h, tn) + part * 16 * a.st[z][3], a.st[z][3], raw[z]);
+  }
   if (a.cu != nullptr) {
     int t0, h0;
-    token_head(a, min(idx0 / L, a.rows - 1), t0, h0);
+    token_head(a, first, t0, h0);
     b = walk_sequence(a.cu, a.batch, block_first_sequence(a.cu, a.batch, t0), t);
     if (b >= a.batch) {  // behind the last sequence
       on = false;
@@ -120,8 +179,8 @@ __global__ void __launch_bounds__(128) append_kernel(const RowArgs a) {
     i = t - start;
     if (i < 0) on = false;  // a row before the first sequence
   } else {
-    b = t / a.n;
-    i = t - b * a.n;
+    b = tb;
+    i = tn;
     n_new = a.n;
   }
   const int len = __ldg(a.lens + b);
@@ -131,27 +190,17 @@ __global__ void __launch_bounds__(128) append_kernel(const RowArgs a) {
     report(a.err, FA2_ERR_SHAPE);
     on = false;
   }
-  int64_t page = 0;
-  int row = 0;
+  int page = 0, row = 0;
   if (on) on = find_row(a, b, pos, page, row);
-  float f[2][16] = {};
-  if (on) {
-#pragma unroll
-    for (int z = 0; z < 2; ++z) {
-      const int64_t bi = a.cu != nullptr ? 0 : b, ni = a.cu != nullptr ? t : i;
-      load16<BF16, VEC>(a.x[z] + bi * a.st[z][0] + h * a.st[z][1] + ni * a.st[z][2] + part * 16 * a.st[z][3],
-                        a.st[z][3], f[z]);
-    }
-  }
 #pragma unroll
   for (int z = 0; z < 2; ++z) {
-    const float scale = row_scale<L>(f[z]);  // shuffles: all lanes
+    float f[16];
+    floats16<BF16>(raw[z], f);
+    const float scale = row_scale<L, BF16>(raw[z]);  // shuffles: all lanes
     if (on) {
-      const int64_t* st = z ? a.c.v_st : a.c.k_st;
-      const int64_t* sst = z ? a.c.vs_st : a.c.ks_st;
-      uint8_t* dst = const_cast<uint8_t*>(z ? a.c.v : a.c.k) + page * st[0] + row * st[1] + h * st[2] + part * 16;
-      *reinterpret_cast<uint4*>(dst) = codes16(f[z], scale);
-      if (part == 0) const_cast<float*>(z ? a.c.vs : a.c.ks)[page * sst[0] + row * sst[1] + h * sst[2]] = scale;
+      uint8_t* dst = const_cast<uint8_t*>(z ? a.c.v : a.c.k) + codes_at(a.c, z != 0, page, row, h) + part * 16;
+      *reinterpret_cast<uint4*>(dst) = codes16(f, scale);
+      if (part == 0) const_cast<float*>(z ? a.c.vs : a.c.ks)[scale_at(a.c, z != 0, page, row, h)] = scale;
     }
   }
 }
@@ -159,28 +208,25 @@ __global__ void __launch_bounds__(128) append_kernel(const RowArgs a) {
 template <int D, bool BF16>
 __global__ void __launch_bounds__(128) read_kernel(const RowArgs a) {
   constexpr int L = D / 16;
-  const int64_t idx0 = static_cast<int64_t>(blockIdx.x) * 128;
-  const int64_t row_id = (idx0 + threadIdx.x) / L;
-  const int part = threadIdx.x % L;
+  constexpr int ROWS = 128 / L;  // of a block
+  const int first = static_cast<int>(blockIdx.x) * ROWS;
+  const int part = threadIdx.x % L, row_id = first + static_cast<int>(threadIdx.x) / L;
   int t, h, t0, h0;
   token_head(a, min(row_id, a.rows - 1), t, h);
-  token_head(a, min(idx0 / L, a.rows - 1), t0, h0);
+  token_head(a, first, t0, h0);
   const int b = walk_sequence(a.cu, a.batch, block_first_sequence(a.cu, a.batch, t0), t);
   if (row_id >= a.rows || b >= a.batch) return;
   const int pos = t - __ldg(a.cu + b);
   if (pos < 0) return;
-  int64_t page = 0;
-  int row = 0;
+  int page = 0, row = 0;
   const bool on = find_row(a, b, pos, page, row);
   uint4 w[2] = {};
   float scale[2] = {};
   if (on) {
 #pragma unroll
     for (int z = 0; z < 2; ++z) {
-      const int64_t* st = z ? a.c.v_st : a.c.k_st;
-      const int64_t* sst = z ? a.c.vs_st : a.c.ks_st;
-      w[z] = *reinterpret_cast<const uint4*>((z ? a.c.v : a.c.k) + page * st[0] + row * st[1] + h * st[2] + part * 16);
-      scale[z] = (z ? a.c.vs : a.c.ks)[page * sst[0] + row * sst[1] + h * sst[2]];
+      w[z] = *reinterpret_cast<const uint4*>((z ? a.c.v : a.c.k) + codes_at(a.c, z != 0, page, row, h) + part * 16);
+      scale[z] = (z ? a.c.vs : a.c.ks)[scale_at(a.c, z != 0, page, row, h)];
     }
   }
 #pragma unroll
@@ -194,7 +240,7 @@ __global__ void __launch_bounds__(128) read_kernel(const RowArgs a) {
       o[2 * i] = x2_of_floats<BF16>(lo.x * scale[z], lo.y * scale[z]);
       o[2 * i + 1] = x2_of_floats<BF16>(hi.x * scale[z], hi.y * scale[z]);
     }
-    uint16_t* dst = const_cast<uint16_t*>(a.x[z]) + row_id * D + part * 16;
+    uint16_t* dst = const_cast<uint16_t*>(a.x[z]) + static_cast<int64_t>(row_id) * D + part * 16;
     *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
     *reinterpret_cast<uint4*>(dst + 8) = make_uint4(o[4], o[5], o[6], o[7]);
   }
@@ -202,9 +248,8 @@ __global__ void __launch_bounds__(128) read_kernel(const RowArgs a) {
 
 template <int D>
 int launch_append(const RowArgs& a, bool bf, bool vec, cudaStream_t s) {
-  const int64_t blocks = (a.rows * (D / 16) + 127) / 128;
-  if (blocks > 0x7fffffffll) return FA2_ERR_SHAPE;
-  const unsigned g = static_cast<unsigned>(blocks);
+  constexpr int ROWS = 128 / (D / 16);
+  const unsigned g = (static_cast<unsigned>(a.rows) + ROWS - 1) / ROWS;
   if (bf) {
     if (vec) append_kernel<D, true, true><<<g, 128, 0, s>>>(a);
     else append_kernel<D, true, false><<<g, 128, 0, s>>>(a);
@@ -217,9 +262,8 @@ int launch_append(const RowArgs& a, bool bf, bool vec, cudaStream_t s) {
 
 template <int D>
 int launch_read(const RowArgs& a, bool bf, cudaStream_t s) {
-  const int64_t blocks = (a.rows * (D / 16) + 127) / 128;
-  if (blocks > 0x7fffffffll) return FA2_ERR_SHAPE;
-  const unsigned g = static_cast<unsigned>(blocks);
+  constexpr int ROWS = 128 / (D / 16);
+  const unsigned g = (static_cast<unsigned>(a.rows) + ROWS - 1) / ROWS;
   if (bf) read_kernel<D, true><<<g, 128, 0, s>>>(a);
   else read_kernel<D, false><<<g, 128, 0, s>>>(a);
   return launch_status();
@@ -253,7 +297,8 @@ int fa2_kv8_append_sm100_check(const Fa2Kv8AppendParams* p) {
   const int rc = check_cache(p->cache);
   if (rc != FA2_OK) return rc;
   if (p->batch < 1 || p->seqlen < 0 || p->pages_per_seq < 1) return FA2_ERR_SHAPE;
-  if (static_cast<int64_t>(p->batch) * (p->cu_seqlens != nullptr ? 1 : p->seqlen) > 0x7fffffffll) return FA2_ERR_SHAPE;
+  // Rows (tokens x heads) are counted in 31 bits.
+  if (static_cast<int64_t>(p->cu_seqlens != nullptr ? 1 : p->batch) * p->seqlen > 0x7fff0000ll / p->cache.heads_kv) return FA2_ERR_SHAPE;
   if (p->dtype != FA2_DTYPE_FP16 && p->dtype != FA2_DTYPE_BF16) return FA2_ERR_DTYPE;
   return FA2_OK;
 }
@@ -279,7 +324,12 @@ int fa2_kv8_append_sm100(const Fa2Kv8AppendParams* p, void* stream) {
   a.batch = p->batch;
   a.n = p->seqlen;
   const int64_t tokens = p->cu_seqlens != nullptr ? p->seqlen : static_cast<int64_t>(p->batch) * p->seqlen;
-  a.rows = tokens * p->cache.heads_kv;
+  a.rows = static_cast<int>(tokens * p->cache.heads_kv);
+  a.by_heads = divisor(p->cache.heads_kv);
+  a.by_n = divisor(p->seqlen);
+  for (int z = 0; z < 2; ++z) {
+    for (int i = 0; i < 3; ++i) a.wide = a.wide || a.st[z][i] < -0x7fffffffll || a.st[z][i] > 0x7fffffffll;
+  }
   const int64_t nb = p->cu_seqlens != nullptr ? 1 : p->batch;
   const bool vec = vec_rows(p->k, p->k_in_stride, nb, p->cache.heads_kv, p->seqlen) &&
                    vec_rows(p->v, p->v_in_stride, nb, p->cache.heads_kv, p->seqlen);
@@ -299,7 +349,7 @@ int fa2_kv8_read_sm100_check(const Fa2Kv8ReadParams* p) {
   }
   const int rc = check_cache(p->cache);
   if (rc != FA2_OK) return rc;
-  if (p->batch < 1 || p->total < 0 || p->pages_per_seq < 1) return FA2_ERR_SHAPE;
+  if (p->batch < 1 || p->total < 0 || p->pages_per_seq < 1 || p->total > 0x7fff0000 / p->cache.heads_kv) return FA2_ERR_SHAPE;
   if (p->dtype != FA2_DTYPE_FP16 && p->dtype != FA2_DTYPE_BF16) return FA2_ERR_DTYPE;
   if (!aligned16(p->k_out) || !aligned16(p->v_out)) return FA2_ERR_LAYOUT;
   return FA2_OK;
@@ -320,7 +370,8 @@ int fa2_kv8_read_sm100(const Fa2Kv8ReadParams* p, void* stream) {
   a.pages_per_seq = p->pages_per_seq;
   a.batch = p->batch;
   a.n = p->total;
-  a.rows = static_cast<int64_t>(p->total) * p->cache.heads_kv;
+  a.rows = p->total * p->cache.heads_kv;
+  a.by_heads = divisor(p->cache.heads_kv);
   const bool bf = p->dtype == FA2_DTYPE_BF16;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (p->cache.head_dim) {

@@ -25,7 +25,7 @@ struct Cache {
   int heads_kv;
   // The same strides in 32 bits (page strides of codes in 16-byte units), for offsets that are one
   // widening product each.
-  int k_page16, v_page16, ks_page, vs_page, k_row, v_row, ks_row, vs_row;
+  int k_page16, v_page16, ks_page, vs_page, k_row, v_row, ks_row, vs_row, k_head, v_head, ks_head, vs_head;
 };
 
 __device__ __forceinline__ int page_of(const Cache& c, int pos) {
@@ -109,7 +109,29 @@ __device__ __forceinline__ int walk_sequence(const int* cu, int batch, int b, in
   return b;
 }
 
+// n / d by a multiplication, 0 <= n < 2^31: hi(n mul) >> shift with mul = 2^(31 + s) / d + 1, d <= 2^s
+// (too large by less than n 2^-(31 + s) < 1 / d).
+struct Divisor {
+  int d;
+  uint32_t mul;
+  int shift;
+};
+__device__ __forceinline__ int divide(const Divisor& v, int n) {
+  return v.d == 1 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), v.mul) >> v.shift);
+}
+
 // ------------------------------------------------------------------------------------ host
+inline Divisor divisor(int d) {
+  Divisor v{d, 0, 0};
+  if (d > 1) {
+    int log = 1;
+    while ((1ll << log) < d) ++log;
+    v.mul = static_cast<uint32_t>((1ull << (31 + log)) / static_cast<uint64_t>(d) + 1);
+    v.shift = log - 1;
+  }
+  return v;
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 inline bool page_size_ok(int n) { return n == 16 || n == 32 || n == 64 || (n >= 128 && n % 128 == 0); }
@@ -164,6 +186,12 @@ inline Cache device_cache(const Fa2Kv8Cache& c) {
   d.v_row = static_cast<int>(c.v_stride[1]);
   d.ks_row = static_cast<int>(c.ks_stride[1]);
   d.vs_row = static_cast<int>(c.vs_stride[1]);
+  if (c.heads_kv > 1) {
+    d.k_head = static_cast<int>(c.k_stride[2]);
+    d.v_head = static_cast<int>(c.v_stride[2]);
+    d.ks_head = static_cast<int>(c.ks_stride[2]);
+    d.vs_head = static_cast<int>(c.vs_stride[2]);
+  }
   return d;
 }
 
