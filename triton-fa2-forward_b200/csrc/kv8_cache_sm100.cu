@@ -67,11 +67,12 @@ __device__ __forceinline__ const uint16_t* row_at(const RowArgs& a, int z, int b
          static_cast<int64_t>(n) * static_cast<int>(a.st[z][2]);
 }
 
-// 16 values of a row as they are in memory, and as floats.
-template <bool VEC>
+// A lane's 16 values of a row, as they are in memory and as floats: 8 in each half, so that the lanes
+// of a row ask for (and write) consecutive bytes.
+template <int D, bool VEC>
 __device__ __forceinline__ void load16(const uint16_t* x, int64_t d_stride, uint32_t (&w)[8]) {
   if constexpr (VEC) {
-    const uint4 w0 = __ldcs(reinterpret_cast<const uint4*>(x)), w1 = __ldcs(reinterpret_cast<const uint4*>(x) + 1);
+    const uint4 w0 = __ldcs(reinterpret_cast<const uint4*>(x)), w1 = __ldcs(reinterpret_cast<const uint4*>(x + D / 2));
     w[0] = w0.x;
     w[1] = w0.y;
     w[2] = w0.z;
@@ -83,7 +84,8 @@ __device__ __forceinline__ void load16(const uint16_t* x, int64_t d_stride, uint
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      w[i] = static_cast<uint32_t>(x[2 * i * d_stride]) | (static_cast<uint32_t>(x[(2 * i + 1) * d_stride]) << 16);
+      const int at = i < 4 ? 2 * i : D / 2 + 2 * i - 8;
+      w[i] = static_cast<uint32_t>(x[at * d_stride]) | (static_cast<uint32_t>(x[(at + 1) * d_stride]) << 16);
     }
   }
 }
@@ -164,7 +166,7 @@ __global__ void __launch_bounds__(128) append_kernel(const RowArgs a) {
   const int tb = a.cu != nullptr ? 0 : divide(a.by_n, t), tn = a.cu != nullptr ? t : t - tb * a.n;
 #pragma unroll
   for (int z = 0; z < 2; ++z) {
-    load16<VEC>(row_at(a, z, tb, h, tn) + part * 16 * a.st[z][3], a.st[z][3], raw[z]);
+    load16<D, VEC>(row_at(a, z, tb, h, tn) + part * 8 * a.st[z][3], a.st[z][3], raw[z]);
   }
   if (a.cu != nullptr) {
     int t0, h0;
@@ -198,8 +200,10 @@ __global__ void __launch_bounds__(128) append_kernel(const RowArgs a) {
     floats16<BF16>(raw[z], f);
     const float scale = row_scale<L, BF16>(raw[z]);  // shuffles: all lanes
     if (on) {
-      uint8_t* dst = const_cast<uint8_t*>(z ? a.c.v : a.c.k) + codes_at(a.c, z != 0, page, row, h) + part * 16;
-      *reinterpret_cast<uint4*>(dst) = codes16(f, scale);
+      uint8_t* dst = const_cast<uint8_t*>(z ? a.c.v : a.c.k) + codes_at(a.c, z != 0, page, row, h) + part * 8;
+      const uint4 w = codes16(f, scale);
+      *reinterpret_cast<uint2*>(dst) = make_uint2(w.x, w.y);
+      *reinterpret_cast<uint2*>(dst + D / 2) = make_uint2(w.z, w.w);
       if (part == 0) const_cast<float*>(z ? a.c.vs : a.c.ks)[scale_at(a.c, z != 0, page, row, h)] = scale;
     }
   }
@@ -219,30 +223,33 @@ __global__ void __launch_bounds__(128) read_kernel(const RowArgs a) {
   const int pos = t - __ldg(a.cu + b);
   if (pos < 0) return;
   int page = 0, row = 0;
-  const bool on = find_row(a, b, pos, page, row);
-  uint4 w[2] = {};
+  uint2 w[2][2] = {};
   float scale[2] = {};
-  if (on) {
+  if (find_row(a, b, pos, page, row)) {
 #pragma unroll
     for (int z = 0; z < 2; ++z) {
-      w[z] = *reinterpret_cast<const uint4*>((z ? a.c.v : a.c.k) + codes_at(a.c, z != 0, page, row, h) + part * 16);
+      const uint8_t* src = (z ? a.c.v : a.c.k) + codes_at(a.c, z != 0, page, row, h) + part * 8;
+      w[z][0] = __ldcs(reinterpret_cast<const uint2*>(src));
+      w[z][1] = __ldcs(reinterpret_cast<const uint2*>(src + D / 2));
       scale[z] = (z ? a.c.vs : a.c.ks)[scale_at(a.c, z != 0, page, row, h)];
     }
   }
 #pragma unroll
   for (int z = 0; z < 2; ++z) {
-    const uint32_t c[4] = {w[z].x, w[z].y, w[z].z, w[z].w};
-    uint32_t o[8];
+    uint16_t* dst = const_cast<uint16_t*>(a.x[z]) + static_cast<int64_t>(row_id) * D + part * 8;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 lo = float2_of_f16x2(f16x2_of_e4m3x2(static_cast<uint16_t>(c[i])));
-      const float2 hi = float2_of_f16x2(f16x2_of_e4m3x2(static_cast<uint16_t>(c[i] >> 16)));
-      o[2 * i] = x2_of_floats<BF16>(lo.x * scale[z], lo.y * scale[z]);
-      o[2 * i + 1] = x2_of_floats<BF16>(hi.x * scale[z], hi.y * scale[z]);
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t c[2] = {w[z][i].x, w[z][i].y};
+      uint32_t o[4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float2 lo = float2_of_f16x2(f16x2_of_e4m3x2(static_cast<uint16_t>(c[j])));
+        const float2 hi = float2_of_f16x2(f16x2_of_e4m3x2(static_cast<uint16_t>(c[j] >> 16)));
+        o[2 * j] = x2_of_floats<BF16>(lo.x * scale[z], lo.y * scale[z]);
+        o[2 * j + 1] = x2_of_floats<BF16>(hi.x * scale[z], hi.y * scale[z]);
+      }
+      *reinterpret_cast<uint4*>(dst + i * (D / 2)) = make_uint4(o[0], o[1], o[2], o[3]);
     }
-    uint16_t* dst = const_cast<uint16_t*>(a.x[z]) + static_cast<int64_t>(row_id) * D + part * 16;
-    *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
-    *reinterpret_cast<uint4*>(dst + 8) = make_uint4(o[4], o[5], o[6], o[7]);
   }
 }
 
