@@ -112,7 +112,9 @@ struct Cut {
 // device. A (sequence, head, block) that lies in one worker's share is written as the result; one
 // that is cut leaves a partial result for each share (a worker has at most two: where its share
 // begins and where it ends) and the merge kernel puts them together in the line's order.
-// A tile costs 1, or 2 where a CTA has two different 128-row tiles to do for it.
+// A tile of few rows costs 1. In the 256-row kernel it costs 4, or 3 where a CTA has one 128-row tile of
+// rows to do for it (2.35 and 1.7 us), and a block adds what its start and end take (10 us: 16) where
+// the shares are long enough for that to matter.
 struct Line {
   // Tiles and tile cost of row block rb of sequence s, and the sum over a sequence's blocks.
   __device__ static int blocks(const AttnArgs& a, const Seq& s) { return (s.n_q * a.group + a.block - 1) / a.block; }
@@ -121,17 +123,23 @@ struct Line {
     return (keys_end(a, s, row0, min(a.block, rows - row0)) + 127) / 128;
   }
   __device__ static int tile_cost(const AttnArgs& a, const Seq& s, int rb) {
-    return a.block == 256 && s.n_q * a.group - rb * 256 > 128 ? 2 : 1;
+    return a.block < 256 ? 1 : s.n_q * a.group - rb * 256 > 128 ? 4 : 3;
   }
-  __device__ static int head_cost(const AttnArgs& a, const Seq& s) {
-    int n = 0;
-    for (int rb = 0; rb < blocks(a, s); ++rb) n += tiles(a, s, rb) * tile_cost(a, s, rb);
-    return n;
+  // A kv head's tiles (cost) and blocks that have any.
+  __device__ static void head_cost(const AttnArgs& a, const Seq& s, int& tiles_cost, int& n_blocks) {
+    tiles_cost = n_blocks = 0;
+    for (int rb = 0; rb < blocks(a, s); ++rb) {
+      const int n = tiles(a, s, rb);
+      tiles_cost += n * tile_cost(a, s, rb);
+      n_blocks += n > 0 ? 1 : 0;
+    }
   }
-  // The workers that get something: with two cost units each at least, every share that begins or
-  // ends inside a block holds one of its tiles.
-  __device__ static int workers(const AttnArgs& a, int total) {
-    return min(a.workers, a.block == 256 ? (total + 1) / 2 : total);
+  // From the tiles' cost: the workers that get something, and a block's own cost. Every share is at
+  // least as long as a block's own cost and a tile, so one that begins or ends inside a block but for
+  // its first tile holds one of its tiles.
+  __device__ static int workers(const AttnArgs& a, int cost) { return min(a.workers, a.block < 256 ? cost : max(1, cost / 4)); }
+  __device__ static int block_cost(const AttnArgs& a, int cost) {
+    return a.block < 256 ? 0 : min(16, max(0, cost / a.workers - 4));
   }
   // Where worker w's share starts, and the worker whose share holds position x.
   __device__ static int start(int w, int workers, int total) {  // w total / workers, in 32 bits
@@ -149,27 +157,39 @@ struct Line {
 // Finds, with a warp, the length of the line, this worker's share of it and a sequence at or before
 // the share's start. Each lane adds up a run of sequences.
 struct Share {
-  int total, p0, p1;  // the line's length; this worker's share
+  int total, workers, block_cost;
+  int p0, p1;         // this worker's share
   int b, start_b;     // the first sequence of the run that holds p0, and where it starts
 };
 __device__ __forceinline__ Share find_share(const AttnArgs& a, int w) {
   const int lane = static_cast<int>(threadIdx.x) & 31, per = (a.batch + 31) / 32;
   const int b0 = min(a.batch, lane * per), b1 = min(a.batch, b0 + per);
-  int own = 0;
+  int own = 0, own_blocks = 0;
 #pragma unroll 1
-  for (int b = b0; b < b1; ++b) own += a.heads_kv * Line::head_cost(a, sequence(a, b));
-  int sum = own;
+  for (int b = b0; b < b1; ++b) {
+    int cost, n;
+    Line::head_cost(a, sequence(a, b), cost, n);
+    own += a.heads_kv * cost;
+    own_blocks += a.heads_kv * n;
+  }
+  int sum = own, sum_blocks = own_blocks;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, sum, o);
-    if (lane >= o) sum += v;
+    const int v = __shfl_up_sync(0xffffffffu, sum, o), n = __shfl_up_sync(0xffffffffu, sum_blocks, o);
+    if (lane >= o) {
+      sum += v;
+      sum_blocks += n;
+    }
   }
   Share r;
-  r.total = __shfl_sync(0xffffffffu, sum, 31);
-  const int workers = Line::workers(a, r.total);
-  r.p0 = w < workers ? Line::start(w, workers, r.total) : 0;
-  r.p1 = w < workers ? Line::start(w + 1, workers, r.total) : 0;
-  const int before = sum - own;
+  const int cost = __shfl_sync(0xffffffffu, sum, 31);
+  r.workers = Line::workers(a, cost);
+  r.block_cost = Line::block_cost(a, cost);
+  r.total = cost + r.block_cost * __shfl_sync(0xffffffffu, sum_blocks, 31);
+  r.p0 = w < r.workers ? Line::start(w, r.workers, r.total) : 0;
+  r.p1 = w < r.workers ? Line::start(w + 1, r.workers, r.total) : 0;
+  own += r.block_cost * own_blocks;
+  const int before = sum + r.block_cost * sum_blocks - own;
   const uint32_t at = __ballot_sync(0xffffffffu, before <= r.p0 && r.p0 < before + own);
   const int from = at != 0 ? __ffs(at) - 1 : 0;
   r.b = __shfl_sync(0xffffffffu, b0, from);
@@ -181,29 +201,33 @@ __device__ __forceinline__ Share find_share(const AttnArgs& a, int w) {
 struct Block {
   Seq sq;
   int b, h, rb;
-  int at, tiles, cost;  // first position, tiles, cost of each
+  int at, tiles, cost;  // position of the first tile, tiles, cost of each
+  int first;            // position of the block
   // The first tile at or behind position p. A share that begins or ends inside a tile: the tile
   // belongs to the earlier worker.
   __device__ int tile_of(int p) const { return p <= at ? 0 : min(tiles, (p - at + cost - 1) / cost); }
 };
 // The block that holds position p, walking on from sequence b, which starts at `start`.
-__device__ __forceinline__ void find_block(const AttnArgs& a, int p, int& b, int& start, Block& o) {
+__device__ __forceinline__ void find_block(const AttnArgs& a, int block_cost, int p, int& b, int& start, Block& o) {
   int hc;
   while (true) {
     o.sq = sequence(a, b);
-    hc = Line::head_cost(a, o.sq);
+    int n;
+    Line::head_cost(a, o.sq, hc, n);
+    hc += n * block_cost;
     if (p < start + hc * a.heads_kv) break;
     start += hc * a.heads_kv;
     ++b;
   }
   o.b = b;
   o.h = (p - start) / hc;
-  o.at = start + o.h * hc;
+  o.first = start + o.h * hc;
   for (o.rb = 0;; ++o.rb) {
     o.tiles = Line::tiles(a, o.sq, o.rb);
     o.cost = Line::tile_cost(a, o.sq, o.rb);
+    o.at = o.first + (o.tiles > 0 ? block_cost : 0);
     if (p < o.at + o.tiles * o.cost) return;
-    o.at += o.tiles * o.cost;
+    o.first = o.at + o.tiles * o.cost;
   }
 }
 
@@ -228,7 +252,7 @@ struct Pieces {
   __device__ bool next(const AttnArgs& a, Piece& o) {
     while (p < s.p1) {
       Block k;
-      find_block(a, p, s.b, s.start_b, k);
+      find_block(a, s.block_cost, p, s.b, s.start_b, k);
       o.sq = k.sq;
       o.b = k.b;
       o.h = k.h;
@@ -238,17 +262,17 @@ struct Pieces {
       const int row0 = o.rb * a.block;
       o.kend = keys_end(a, o.sq, row0, min(a.block, o.sq.n_q * a.group - row0));
       if (p == s.p0) {
-        const int workers = Line::workers(a, s.total), before = w > 0 ? Line::start(w - 1, workers, s.total) : 0;
+        const int before = w > 0 ? Line::start(w - 1, s.workers, s.total) : 0;
         Cut c{};
         if (o.tiles > 0 && o.t0 > 0 && k.tile_of(before) == 0) {
-          // (A tile is its start's holder's. Shares of two units and more between hold one each.)
-          c.n_parts = Line::holder(k.at + (k.tiles - 1) * k.cost, workers, s.total) - w + 2;
+          // (A tile is its start's holder's.)
+          c.n_parts = Line::holder(k.at + (k.tiles - 1) * k.cost, s.workers, s.total) - w + 2;
           c.b = o.b;
           c.h = o.h;
           c.row0 = row0;
           c.q0 = o.sq.q0;
           c.n_q = o.sq.n_q;
-          c.first_slot = 2 * (w - 1) + (before >= k.at ? 0 : 1);
+          c.first_slot = 2 * (w - 1) + (before >= k.first ? 0 : 1);
         }
         a.cuts[w] = c;
       }

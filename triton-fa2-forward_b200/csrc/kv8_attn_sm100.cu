@@ -538,13 +538,33 @@ __global__ void __launch_bounds__(DEC_WARPS * 32, DEC_CTAS) decode_kernel(const 
 
 // ------------------------------------------------------------------ merge of the partial results
 // o = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max) over a cut block's parts, in the line's order, a
-// warp a row: CTA (x, y) has the rows [8 y, 8 y + 8) of the block that share x + 1 is the first to cut.
+// warp a row (four rows side by side in the 256-row kernel): CTA (x, y) has 4 R rows of the block that
+// share x + 1 is the first to cut. Loads wait for no other part's: with a branch around each the
+// merge of 32 parts alone took 14 us.
 // The last ZERO_CTAS write zeros for the blocks without a tile, which no worker has.
 constexpr int ZERO_CTAS = 16;
-constexpr int MERGE_ROWS = 8;
+constexpr int merge_rows(int block) { return block < 256 ? 4 : 16; }
 
-template <int D, bool BF16>
+template <int N>
+__device__ __forceinline__ void load_floats(const float* p, float (&v)[N]) {
+  if constexpr (N == 4) {
+    const float4 x = *reinterpret_cast<const float4*>(p);
+    v[0] = x.x;
+    v[1] = x.y;
+    v[2] = x.z;
+    v[3] = x.w;
+  } else if constexpr (N == 2) {
+    const float2 x = *reinterpret_cast<const float2*>(p);
+    v[0] = x.x;
+    v[1] = x.y;
+  } else {
+    v[0] = *p;
+  }
+}
+
+template <int D, bool BF16, int R>
 __global__ void __launch_bounds__(128) merge_kernel(const AttnArgs a) {
+  constexpr int MERGE_ROWS = 4 * R;  // a warp's: row_first + warp + 4 k
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row_first = static_cast<int>(blockIdx.y) * MERGE_ROWS;
   const int w = static_cast<int>(blockIdx.x) + 1;
@@ -575,33 +595,61 @@ __global__ void __launch_bounds__(128) merge_kernel(const AttnArgs a) {
     return static_cast<int64_t>(i == 0 ? cut.first_slot : 2 * (w - 1 + i)) * a.block + r;
   };
   if (cut.n_parts == 0) return;
-  for (int r = row_first + warp; r < min(rows, row_first + MERGE_ROWS); r += 4) {
-    float mx = -INFINITY;
-    for (int i = lane; i < cut.n_parts; i += 32) mx = fmaxf(mx, a.lse_part[part(i, r)]);
+  const int r0 = row_first + warp;
+  float mx[R], sum[R] = {}, acc[R][PER] = {};
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    float acc[PER] = {}, sum = 0.0f;
-    for (int i0 = 0; i0 < cut.n_parts; i0 += 32) {
-      const float v = i0 + lane < cut.n_parts ? a.lse_part[part(i0 + lane, r)] : -INFINITY;
-      const float f = v == -INFINITY ? 0.0f : exp2f(v - (mx == -INFINITY ? 0.0f : mx));  // a NaN stays one
-      const int n = min(32, cut.n_parts - i0);
-#pragma unroll 4
-      for (int i = 0; i < n; ++i) {
-        const float fi = __shfl_sync(0xffffffffu, f, i);
-        if (on && fi != 0.0f) {
-          const float* src = a.o_part + part(i0 + i, r) * D + lane * PER;
+  for (int k = 0; k < R; ++k) mx[k] = -INFINITY;
+  for (int i = lane; i < cut.n_parts; i += 32) {
 #pragma unroll
-          for (int j = 0; j < PER; ++j) acc[j] = fmaf(fi, src[j], acc[j]);
+    for (int k = 0; k < R; ++k) {
+      if (r0 + 4 * k < rows) mx[k] = fmaxf(mx[k], a.lse_part[part(i, r0 + 4 * k)]);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < R; ++k) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], o));
+  }
+  for (int i0 = 0; i0 < cut.n_parts; i0 += 32) {
+    float f[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      const float v = i0 + lane < cut.n_parts && r0 + 4 * k < rows ? a.lse_part[part(i0 + lane, r0 + 4 * k)] : -INFINITY;
+      f[k] = v == -INFINITY ? 0.0f : exp2f(v - (mx[k] == -INFINITY ? 0.0f : mx[k]));  // a NaN stays one
+    }
+    const int n = min(32, cut.n_parts - i0);
+    constexpr int AT_ONCE = R == 1 ? 8 : 2;
+    for (int i = 0; i < n; i += AT_ONCE) {
+      float v[AT_ONCE][R][PER];
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+          const int64_t at = part(i0 + min(i + u, n - 1), min(r0 + 4 * k, rows - 1)) * D + (on ? lane * PER : 0);
+          load_floats<PER>(a.o_part + at, v[u][k]);
         }
-        sum += fi;
+      }
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+          const float fi = __shfl_sync(0xffffffffu, f[k], i + u);  // 0 from part n on
+          sum[k] += fi;
+#pragma unroll
+          for (int j = 0; j < PER; ++j) {  // a part without a key has weight 0, and may hold anything
+            acc[k][j] = fi != 0.0f ? fmaf(fi, v[u][k][j], acc[k][j]) : acc[k][j];
+          }
+        }
       }
     }
-    if (on) {
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      uint16_t* dst = o_row(a, sq, cut.b, cut.h, cut.row0 + r) + lane * PER;
+  }
 #pragma unroll
-      for (int j = 0; j < PER; ++j) dst[j] = x1_of_float<BF16>(acc[j] * inv);
-    }
+  for (int k = 0; k < R; ++k) {
+    if (!on || r0 + 4 * k >= rows) continue;
+    const float inv = sum[k] == 0.0f ? 0.0f : 1.0f / sum[k];
+    uint16_t* dst = o_row(a, sq, cut.b, cut.h, cut.row0 + r0 + 4 * k) + lane * PER;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) dst[j] = x1_of_float<BF16>(acc[k][j] * inv);
   }
 }
 
@@ -620,12 +668,27 @@ Plan plan(const Fa2Kv8AttnParams* p) {
   const int64_t rows = static_cast<int64_t>(p->seqlen_q) * (p->heads_q / p->cache.heads_kv);
   r.block = rows <= 8 ? 8 : rows <= 16 ? 16 : 256;
   const int64_t units = static_cast<int64_t>(p->batch) * p->cache.heads_kv * std::max<int64_t>(1, (rows + r.block - 1) / r.block);
-  // One wave: DEC_SHARES CTAs, or one of the 256-row kernel, on each of 148 SMs; with fewer (sequence,
-  // head, block)s than that a multiple of their number, so that equal ones are cut alike.
+  // One wave: DEC_SHARES CTAs, or one of the 256-row kernel, on each of 148 SMs.
   const int64_t most = r.block == 256 ? 148 : 148 * DEC_SHARES;
-  const int64_t tiles = units * ((static_cast<int64_t>(p->max_seqlen_k) + 127) / 128);
-  int64_t w = p->num_splits > 0 ? units * p->num_splits : units < most && r.block < 256 ? most / units * units : most;
-  if (w > most && p->num_splits <= 0) w = most;
+  const int64_t per_unit = (static_cast<int64_t>(p->max_seqlen_k) + 127) / 128, tiles = units * per_unit;
+  int64_t w = most;
+  if (p->num_splits > 0) {
+    w = units * p->num_splits;
+  } else if (units <= most) {
+    // With fewer (sequence, head, block)s than that a multiple of their number cuts equal ones alike.
+    const int64_t alike = most / units * units;
+    if (r.block < 256) {
+      // Three tiles a share at least (8 heads of 8192 keys: 15 us with three or four, 16 with two, 18
+      // with fewer).
+      const int64_t least = std::max<int64_t>(3, (per_unit + most / units - 1) / (most / units));
+      w = std::max<int64_t>(1, (per_unit + least - 1) / least) * units;
+    } else {
+      // Shares that hold one whole block each need no merge (15 us), and those of one block alone start
+      // and end one piece less (10 us): taken where a CTA has at most as much more to do.
+      const int64_t more = (tiles + alike - 1) / alike - tiles / most;
+      if (more <= (alike == units ? 6 : 3)) w = alike;
+    }
+  }
   if (w > 148 * 16) w = 148 * 16;
   if (w > tiles) w = tiles;
   r.workers = static_cast<int>(w < 1 ? 1 : w);
@@ -656,12 +719,15 @@ int check_core(const Fa2Kv8AttnParams* p) {
   for (int i = 0; i < 3; ++i) {
     if (n[i] > 1 && ((p->q_stride[i] | p->o_stride[i]) & 7) != 0) return FA2_ERR_LAYOUT;
   }
-  // Row numbers, the line of tiles (two cost units each) and the grids stay in 31 bits.
+  // Row numbers, the line of tiles (four cost units each, and 16 a block) and the grids stay in 31 bits.
   const int64_t rows = static_cast<int64_t>(p->seqlen_q) * (p->heads_q / p->cache.heads_kv);
   if (rows > (1ll << 30) || static_cast<int64_t>(p->batch) * p->cache.heads_kv > (1ll << 26)) return FA2_ERR_SHAPE;
-  const int64_t units = static_cast<int64_t>(p->batch) * p->cache.heads_kv * ((rows + 255) / 256);
-  const int64_t tiles = (static_cast<int64_t>(p->max_seqlen_k) + 127) / 128;
-  if (units > (1ll << 26) || units * tiles > (1ll << 29)) return FA2_ERR_SHAPE;
+  int64_t blocks = static_cast<int64_t>(p->batch) * ((rows + 255) / 256);
+  if (p->cu_seqlens_q != nullptr) {
+    blocks = std::min(blocks, static_cast<int64_t>(p->total_q) * (p->heads_q / p->cache.heads_kv) / 256 + p->batch);
+  }
+  const int64_t units = blocks * p->cache.heads_kv, tiles = (static_cast<int64_t>(p->max_seqlen_k) + 127) / 128;
+  if (units > (1ll << 25) || units * tiles > (1ll << 28)) return FA2_ERR_SHAPE;
   return FA2_OK;
 }
 
@@ -682,12 +748,14 @@ int launch_merge(const AttnArgs& a, cudaStream_t s) {
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(a.workers - 1 + ZERO_CTAS), (a.block + MERGE_ROWS - 1) / MERGE_ROWS);
+  cfg.gridDim = dim3(static_cast<unsigned>(a.workers - 1 + ZERO_CTAS), a.block / merge_rows(a.block));
   cfg.blockDim = dim3(128);
   cfg.stream = s;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, merge_kernel<D, BF16>, a) == cudaSuccess ? FA2_OK : FA2_ERR_LAUNCH;
+  const cudaError_t e = a.block < 256 ? cudaLaunchKernelEx(&cfg, merge_kernel<D, BF16, merge_rows(8) / 4>, a)
+                                      : cudaLaunchKernelEx(&cfg, merge_kernel<D, BF16, merge_rows(256) / 4>, a);
+  return e == cudaSuccess ? FA2_OK : FA2_ERR_LAUNCH;
 }
 
 template <int D, bool BF16>

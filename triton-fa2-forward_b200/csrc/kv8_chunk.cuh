@@ -257,6 +257,12 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
         mbar_arrive(bar(CB_PF + i % CH_PIECES));
       }
       __syncwarp();
+      const int first = o.rb * 256, end = more ? min(first + 256, o.sq.n_q * a.group) : 0;
+      for (int r = first + lane; r < end; r += 32) {  // its queries, towards L2
+        const uint16_t* src = q_row(a, o.sq, o.b, o.h, r);
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(src));
+        if constexpr (D > 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + 64));
+      }
     }
   } else if (warp == CH_K_WARP || warp == CH_V_WARP) {
     // -------------------------------------------------------------- codes: pages -> shared memory
@@ -524,25 +530,36 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
       const int tile_row0 = row0 + (dual ? 0 : t * 128), row = tile_row0 + r;
       // Q: a warp's 32 rows as e4m3 terms, 8 lanes (D / 16) a row, 16 values each; every row times the power
       // of two that brings its largest value into [128, 256). Each term is the rounding of what the
-      // terms before leave (an exact difference in fp32).
+      // terms before leave (an exact difference in fp32). The raw values come by asynchronous copies, all
+      // under way at once, to where this lane's first two terms go: it alone reads and overwrites them.
       float row_sc;
       {
         constexpr int LANES = D / 16, STEP = 32 / LANES;  // lanes of a row, rows at a time
         const int part = lane % LANES;
         float* scales = reinterpret_cast<float*>(smem + C::OFF_QS) + t * 128 + q * 32;  // of the warp's rows
         const uint32_t dst = sbase + C::OFF_Q + t * C::TERMS * C::CODES;
-        for (int i = 0; i < LANES; ++i) {  // (all on their way before the first is waited for)
-          const int qr = tile_row0 + q * 32 + i * STEP + lane / LANES;
-          if (qr < rows) asm volatile("prefetch.global.L1 [%0];" ::"l"(q_row(a, o.sq, o.b, o.h, qr) + part * 16));
-        }
+        auto place = [&](int i) -> uint32_t {  // of this lane's part of its row in term 0
+          const int rt = q * 32 + i * STEP + lane / LANES;
+          return dst + rt * 128 + ((part ^ (rt & 7)) << 4);
+        };
 #pragma unroll 2
         for (int i = 0; i < LANES; ++i) {
-          const int rw = i * STEP + lane / LANES, rt = q * 32 + rw, qr = tile_row0 + rt;
-          const bool in = qr < rows;
-          const uint4* src = reinterpret_cast<const uint4*>(q_row(a, o.sq, o.b, o.h, in ? qr : row0) + part * 16);
+          const int qr = tile_row0 + q * 32 + i * STEP + lane / LANES;
+          const uint16_t* src = q_row(a, o.sq, o.b, o.h, qr < rows ? qr : row0) + part * 16;
+          cp_async16(place(i), src, qr < rows);
+          cp_async16(place(i) + C::CODES, src + 8, qr < rows);
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+#pragma unroll 2
+        for (int i = 0; i < LANES; ++i) {
+          const int rw = i * STEP + lane / LANES, rt = q * 32 + rw;
           uint4 v[2];
-          v[0] = in ? __ldg(src) : make_uint4(0, 0, 0, 0);
-          v[1] = in ? __ldg(src + 1) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(v[z].x), "=r"(v[z].y), "=r"(v[z].z), "=r"(v[z].w) : "r"(place(i) + z * C::CODES) : "memory");
+          }
           const uint32_t w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
           float x[16];
           uint32_t top = 0;
@@ -576,9 +593,8 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
                 }
                 y[j] = static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
               }
-              const uint32_t at = dst + term * C::CODES + rt * 128;
-              fa2::st_shared_v4(at + ((part ^ (rt & 7)) << 4), y[0], y[1], y[2], y[3]);
-              if constexpr (D < 32) fa2::st_shared_v4(at + ((1 ^ (rt & 7)) << 4), 0, 0, 0, 0);
+              fa2::st_shared_v4(place(i) + term * C::CODES, y[0], y[1], y[2], y[3]);
+              if constexpr (D < 32) fa2::st_shared_v4(dst + term * C::CODES + rt * 128 + ((1 ^ (rt & 7)) << 4), 0, 0, 0, 0);
             }
           }
         }
