@@ -374,7 +374,12 @@ def test_reports_of_lengths_and_pages():
     for bad in (-1, 6 * 64, 1 << 30):
         out = attention_kvcache_fp8(q, cache, bt, torch.tensor([bad, 200], dtype=torch.int32).cuda(), max_seqlen_k=320)
         reported(_lib.FA2_ERR_SHAPE)
-        assert (out[0] == 0).all() and torch.equal(out[1], attention_kvcache_fp8(q, cache, bt, sl, max_seqlen_k=320)[1])
+        # As if it had no keys. The other sequence's keys may be cut elsewhere than beside a good one (the
+        # sequences share the work as one line), so its sum differs in rounding: both results are
+        # within `tolerance` of the same value, none is promised to have the other's bits.
+        ref, weight, spread, small = serving.attention(q, cache, bt, torch.tensor([0, 200], dtype=torch.int32).cuda())
+        assert (out[0] == 0).all() and (ref[0] == 0).all()
+        assert ((out.double() - ref).abs() <= tolerance(q, weight, spread, small, ref, 200, 8.0)).all()
     for page in (-1, cache.k.shape[0], 1 << 30):
         wrong = bt.clone()
         wrong[1, 1] = page

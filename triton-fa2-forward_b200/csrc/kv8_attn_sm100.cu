@@ -33,7 +33,9 @@ constexpr int DEC_WARPS = 4;
 constexpr int DEC_KEYS = 32;   // of a group
 constexpr int DEC_STAGES = 2;  // 12 warps an SM x one group on its way: 96 KB
 constexpr int DEC_CTAS = 3;    // an SM at most
-constexpr int DEC_SHARES = 2;  // CTAs an SM that the work is shared among
+// CTAs an SM that the work is shared among: two, three where rows of codes are shorter (4 sequences of
+// 65536 keys, D = 128: 91 and 96 us; 48 of up to 8192, D = 64: 30 and 27 us).
+constexpr int dec_shares(int head_dim) { return head_dim > 64 ? 2 : 3; }
 
 template <int D>
 struct Dec {
@@ -668,8 +670,8 @@ Plan plan(const Fa2Kv8AttnParams* p) {
   const int64_t rows = static_cast<int64_t>(p->seqlen_q) * (p->heads_q / p->cache.heads_kv);
   r.block = rows <= 8 ? 8 : rows <= 16 ? 16 : 256;
   const int64_t units = static_cast<int64_t>(p->batch) * p->cache.heads_kv * std::max<int64_t>(1, (rows + r.block - 1) / r.block);
-  // One wave: DEC_SHARES CTAs, or one of the 256-row kernel, on each of 148 SMs.
-  const int64_t most = r.block == 256 ? 148 : 148 * DEC_SHARES;
+  // One wave: dec_shares() CTAs, or one of the 256-row kernel, on each of 148 SMs.
+  const int64_t most = r.block == 256 ? 148 : 148 * dec_shares(p->cache.head_dim);
   const int64_t per_unit = (static_cast<int64_t>(p->max_seqlen_k) + 127) / 128, tiles = units * per_unit;
   int64_t w = most;
   if (p->num_splits > 0) {
