@@ -1,7 +1,7 @@
 // Attention over the 8-bit paged cache for many rows (chunks of prompts): tcgen05 products.
 //
-// Bound by the tensor cores (4 D operations a score) and, inside a step, by the exponentials
-// (16 a clock and SM), the issue slots and shared memory. A CTA owns 256 rows (queries x heads of a
+// Bound by the tensor cores (4 D operations a score) and, inside a step, by the softmax warps' issue
+// slots: an eighth of the exponentials on the FMA pipe instead made it 5% slower. A CTA owns 256 rows (queries x heads of a
 // group) as two 128-row tiles that take turns: while one tile's scores go through the softmax, the
 // tensor core works on the other. With 128 rows or fewer both tiles hold the same rows and take
 // every other 128-key tile, merged at the end. One CTA an SM works through the pieces of its share of

@@ -25,6 +25,7 @@ from .kernel import CAUSAL_ALIGNS, LOG2E, _err_word, _sync_check_enabled, check_
 
 
 _DTYPES = (torch.float16, torch.bfloat16)
+_workspace_bytes = {}  # of attention_kvcache_fp8, by the sizes that it follows from
 
 
 class KVCacheFP8(NamedTuple):
@@ -225,7 +226,7 @@ def attention_kvcache_fp8(q, cache, block_table, cache_seqlens, max_seqlen_k=Non
         return out.zero_()
     bt, sl = _table(block_table), cache_seqlens.contiguous()
     qq, oo = q, out
-    if not _aligned(q) or not _aligned(out):  # layout copy: rows are moved 16 bytes at a time
+    if not _aligned(q) or (out.stride() != q.stride() and not _aligned(out)):  # layout copy: rows are moved 16 bytes at a time
         qq = q.clone(memory_format=torch.contiguous_format)
         oo = torch.empty_like(qq)
     L = _kvlib.lib()
@@ -234,12 +235,16 @@ def attention_kvcache_fp8(q, cache, block_table, cache_seqlens, max_seqlen_k=Non
     tail = (bt.stride(0), 0, pages_per_seq, B, H_q, n_q, q_shape[0] if packed else 0, int(max_seqlen_k),
             dtype == torch.bfloat16, bool(causal), CAUSAL_ALIGNS[causal_align],
             0 if num_splits is None else max(1, int(num_splits)), sm_scale * LOG2E, 0)
-    call = _kvlib.ATTN.pack(*head, 0, 0, *tail)
-    nbytes = L.fa2_kv8_attn_sm100_workspace_bytes(call)
-    if nbytes > 0:
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)  # caching allocator, this stream's
-        call = _kvlib.ATTN.pack(*head, ws.data_ptr(), nbytes, *tail)
-    _launch(L.fa2_kv8_attn_sm100, call, index)
+    sizes = (B, H_q, H_kv, D, n_q, tail[7], tail[11])
+    nbytes = _workspace_bytes.get(sizes)
+    if nbytes is None:
+        nbytes = max(0, L.fa2_kv8_attn_sm100_workspace_bytes(_kvlib.ATTN.pack(*head, 0, 0, *tail)))  # (-1: refused below)
+        if nbytes:
+            if len(_workspace_bytes) >= 4096:
+                _workspace_bytes.clear()
+            _workspace_bytes[sizes] = nbytes
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)  # caching allocator, this stream's
+    _launch(L.fa2_kv8_attn_sm100, _kvlib.ATTN.pack(*head, ws.data_ptr(), nbytes, *tail), index)
     if oo is not out:
         out.copy_(oo)
     return out
