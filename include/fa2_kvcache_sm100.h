@@ -123,7 +123,10 @@ typedef struct Fa2Kv8ReadParams {
 
 /* out = softmax(q k^T * sm_scale + mask) v over the cache. q, o: [B, H_q, N, D], or packed
  * [total, H_q, D] with cu_seqlens_q (the token axis as n). causal_align as in fa2_sm100.h, per
- * sequence. A query that sees no key gets zeros, and so does a sequence whose length is refused. */
+ * sequence. A query that sees no key gets zeros, and so does a sequence whose length is refused. The
+ * sequences of a call share the GPU as one line of work that is cut into equal shares, and partial sums
+ * are joined in its order: the same call gives the same bits, but another batch around a sequence may
+ * cut it elsewhere and change its last bits. */
 typedef struct Fa2Kv8AttnParams {
   Fa2Kv8Cache cache;
   const void* q;
@@ -134,7 +137,8 @@ typedef struct Fa2Kv8AttnParams {
   const int32_t* cache_seqlens;
   const int32_t* cu_seqlens_q;
   int32_t* err_flag;
-  void* workspace; /* fa2_kv8_attn_workspace_bytes() bytes, 16-byte aligned */
+  void* workspace; /* fa2_kv8_attn_sm100_workspace_bytes() bytes, 16-byte aligned; not to be shared
+                    * by calls that may run at the same time */
   int64_t workspace_bytes;
   int64_t block_table_stride;
   int64_t timeout_cycles; /* per-wait limit in SM clocks; <= 0 selects the default (~1 s) */
@@ -147,7 +151,8 @@ typedef struct Fa2Kv8AttnParams {
   int32_t dtype;
   int32_t causal;
   int32_t causal_align;
-  int32_t num_splits; /* 0: chosen from the sizes; else the wanted number of key ranges (1: none) */
+  int32_t num_splits; /* 0: chosen from the sizes; else the CTAs that share the work, for each
+                       * (sequence, kv head, row block): key ranges where those are alike */
   float qk_scale;     /* sm_scale * log2(e), > 0 */
   int32_t reserved;
 } Fa2Kv8AttnParams;
@@ -162,7 +167,8 @@ FA2_API int fa2_kv8_read_sm100_check(const Fa2Kv8ReadParams* p);
 FA2_API int fa2_kv8_read_sm100(const Fa2Kv8ReadParams* p, void* stream);
 
 FA2_API int fa2_kv8_attn_sm100_check(const Fa2Kv8AttnParams* p);
-/* Workspace of the call `p` describes (0: none). Host only; -1 where the check refuses p. */
+/* Workspace of the call `p` describes, which follows from batch, heads, head_dim, seqlen_q, max_seqlen_k
+ * and num_splits. Host only; -1 where the check refuses p (the workspace's own fields aside). */
 FA2_API int64_t fa2_kv8_attn_sm100_workspace_bytes(const Fa2Kv8AttnParams* p);
 FA2_API int fa2_kv8_attn_sm100(const Fa2Kv8AttnParams* p, void* stream);
 

@@ -186,9 +186,11 @@ def attention_kvcache_fp8(q, cache, block_table, cache_seqlens, max_seqlen_k=Non
     block_table: int32 [B, pages_per_seq]; cache_seqlens: int32 [B] keys per sequence, bounded by
     max_seqlen_k (default: pages_per_seq * page_size; a longer one is reported as a device error and
     attends to nothing). The causal mask is per sequence, bottom-right by default (the queries are the
-    last positions). A query that sees no key gets zeros. num_splits: key ranges that run beside one
-    another (None: chosen from the sizes). A query that sees a key of a refused page gets NaN. Returns
-    a tensor like q (rows past cu_seqlens_q[B] are not written), asynchronously.
+    last positions). A query that sees no key gets zeros, one that sees a key of a refused page NaN.
+    num_splits: CTAs that share the work for each (sequence, kv head, block of rows); None: chosen from
+    the sizes. The same call gives the same bits; another batch around a sequence may cut its keys
+    elsewhere and change its last bits. Returns a tensor like q (rows past cu_seqlens_q[B] are not
+    written), asynchronously.
     """
     fields, shape, tensors = _cache_fields(cache)
     q_shape, dtype = q.shape, q.dtype
