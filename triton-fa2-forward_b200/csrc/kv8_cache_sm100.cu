@@ -2,10 +2,16 @@
 // they are written into their pages, and read back. Memory bound both ways: 3 bytes a value and 4
 // a row.
 //
-// A row of D values is held by D / 16 neighbouring lanes, 16 values each (two 16-byte loads, one
-// 16-byte store of codes), the largest magnitude by shuffles among them. A thread has the key's
-// and the value's row of the same token and head: they share the page, and four loads are in
-// flight. Heads run fastest, as the packed tokens have them in memory.
+// A row of D values is held by D / 16 neighbouring lanes, 8 values of each half, so that every load
+// and store of a row is of consecutive bytes (16 values in a piece took 87 us in place of 76 for the
+// reading below: half-filled sectors). The largest magnitude comes by shuffles among them. A thread has
+// the key's and the value's row of the same token and head: they share the page, and four loads are
+// in flight. Heads run fastest, as the packed tokens have them in memory.
+//
+// Measured: append of 17,000 tokens of 8 heads of 128, 103 MB, 25 us (4.1 TB/s, 0.62 of the copy
+// rate): the way from the sums over the table to the page lies before the stores, and a row costs
+// some 300 instructions a lane for its maximum, quotients and codes (with divisions 39 us). Read of
+// 157,000 tokens, 471 MB, 76 us (6.2 TB/s, 0.95); two or four rows a thread were no faster.
 
 #include "kv8_common.cuh"
 
