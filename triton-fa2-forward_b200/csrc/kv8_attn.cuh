@@ -161,6 +161,10 @@ struct Share {
   int p0, p1;         // this worker's share
   int b, start_b;     // the first sequence of the run that holds p0, and where it starts
 };
+// A line whose cost reaches LONGEST_LINE is refused and nothing is done. The host's limits keep every line
+// of sequences that do not overlap below it; sums of query lengths that go back and forth could
+// count the same queries many times.
+constexpr int LONGEST_LINE = (1 << 30) - 1;
 __device__ __forceinline__ Share find_share(const AttnArgs& a, int w) {
   const int lane = static_cast<int>(threadIdx.x) & 31, per = (a.batch + 31) / 32;
   const int b0 = min(a.batch, lane * per), b1 = min(a.batch, b0 + per);
@@ -169,20 +173,25 @@ __device__ __forceinline__ Share find_share(const AttnArgs& a, int w) {
   for (int b = b0; b < b1; ++b) {
     int cost, n;
     Line::head_cost(a, sequence(a, b), cost, n);
-    own += a.heads_kv * cost;
-    own_blocks += a.heads_kv * n;
+    own = min(LONGEST_LINE, own + a.heads_kv * cost);
+    own_blocks = min(LONGEST_LINE, own_blocks + a.heads_kv * n);
   }
   int sum = own, sum_blocks = own_blocks;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int v = __shfl_up_sync(0xffffffffu, sum, o), n = __shfl_up_sync(0xffffffffu, sum_blocks, o);
     if (lane >= o) {
-      sum += v;
-      sum_blocks += n;
+      sum = min(LONGEST_LINE, sum + v);
+      sum_blocks = min(LONGEST_LINE, sum_blocks + n);
     }
   }
   Share r;
   const int cost = __shfl_sync(0xffffffffu, sum, 31);
+  if (cost >= LONGEST_LINE) {
+    report(a.err, FA2_ERR_SHAPE);
+    r = Share{};
+    return r;
+  }
   r.workers = Line::workers(a, cost);
   r.block_cost = Line::block_cost(a, cost);
   r.total = cost + r.block_cost * __shfl_sync(0xffffffffu, sum_blocks, 31);

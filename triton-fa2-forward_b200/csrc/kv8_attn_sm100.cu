@@ -598,7 +598,7 @@ __global__ void __launch_bounds__(128) merge_kernel(const AttnArgs a) {
   auto part = [&](int i, int r) -> int64_t {  // its row
     return static_cast<int64_t>(i == 0 ? cut.first_slot : 2 * (w - 1 + i)) * a.block + r;
   };
-  if (cut.n_parts == 0) return;
+  if (cut.n_parts == 0 || row_first >= rows) return;
   const int r0 = row_first + warp;
   float mx[R], sum[R] = {}, acc[R][PER] = {};
 #pragma unroll
@@ -723,7 +723,8 @@ int check_core(const Fa2Kv8AttnParams* p) {
   for (int i = 0; i < 3; ++i) {
     if (n[i] > 1 && ((p->q_stride[i] | p->o_stride[i]) & 7) != 0) return FA2_ERR_LAYOUT;
   }
-  // Row numbers, the line of tiles (four cost units each, and 16 a block) and the grids stay in 31 bits.
+  // Row numbers and grids stay in 31 bits, the line of tiles (four cost units each, and 16 a block) below
+  // LONGEST_LINE.
   const int64_t rows = static_cast<int64_t>(p->seqlen_q) * (p->heads_q / p->cache.heads_kv);
   if (rows > (1ll << 30) || static_cast<int64_t>(p->batch) * p->cache.heads_kv > (1ll << 26)) return FA2_ERR_SHAPE;
   int64_t blocks = static_cast<int64_t>(p->batch) * ((rows + 255) / 256);
@@ -731,7 +732,7 @@ int check_core(const Fa2Kv8AttnParams* p) {
     blocks = std::min(blocks, static_cast<int64_t>(p->total_q) * (p->heads_q / p->cache.heads_kv) / 256 + p->batch);
   }
   const int64_t units = blocks * p->cache.heads_kv, tiles = (static_cast<int64_t>(p->max_seqlen_k) + 127) / 128;
-  if (units > (1ll << 25) || units * tiles > (1ll << 28)) return FA2_ERR_SHAPE;
+  if (units > (1ll << 24) || units * tiles > (1ll << 27)) return FA2_ERR_SHAPE;
   return FA2_OK;
 }
 
