@@ -286,6 +286,29 @@ def test_attention_packed_queries(dtype, D, num_splits):
     check_attention(q, cache, bt, sl, cu_seqlens_q=cu, max_seqlen_q=301, causal=False, num_splits=num_splits)
 
 
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 64), (torch.float16, 128)])
+def test_attention_long_shares_of_a_ragged_batch(dtype, D):
+    """Shares of many tiles and several blocks, so that a block's own cost counts in the line; new tokens
+    from none to 300, heads in groups of three, so blocks of 256, of 129 to 255 and of fewer rows."""
+    new = [(37 * b * b + 11 * b) % 301 for b in range(40)]
+    lens = [max(n, (97 * b * b + 501) % 2300) if b % 9 else n for b, n in enumerate(new)]
+    cache, bt, sl, _, _, _ = filled(lens, 64, 2, D, dtype, seed=31)
+    cu = torch.tensor([0] + list(torch.tensor(new).cumsum(0)), dtype=torch.int32).cuda()
+    q = randn(sum(new), 6, D, dtype=dtype, seed=32)
+    first = check_attention(q, cache, bt, sl, cu_seqlens_q=cu, max_seqlen_q=300)
+    check_attention(q, cache, bt, sl, cu_seqlens_q=cu, max_seqlen_q=300, causal=False)
+    assert torch.equal(attention_kvcache_fp8(q, cache, bt, sl, cu_seqlens_q=cu, max_seqlen_q=300), first)
+
+
+@pytest.mark.parametrize("N_q", [1, 4, 90])
+def test_attention_many_sequences(N_q):
+    """More sequences than a warp's lanes or the GPU's SMs, every third without a key."""
+    lens = [0 if b % 3 == 2 else 1 + (b * 53) % 400 for b in range(330)]
+    cache, bt, sl, _, _, _ = filled(lens, 16, 1, 32, seed=33)
+    out = check_attention(randn(330, 4, N_q, 32, dtype=torch.bfloat16, seed=34), cache, bt, sl)
+    assert (out[2::3] == 0).all()
+
+
 @pytest.mark.parametrize("N_q", [1, 200])
 def test_attention_sizes_of_values(N_q):
     """Values whose scales span 2^40 from row to row, large and tiny scores, zero rows."""
