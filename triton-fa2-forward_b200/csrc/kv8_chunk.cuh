@@ -1,7 +1,9 @@
 // Attention over the 8-bit paged cache for many rows (chunks of prompts): tcgen05 products.
 //
-// Bound by the tensor cores (4 D operations a score) and, inside a step, by the softmax warps' issue
-// slots: an eighth of the exponentials on the FMA pipe instead made it 5% slower. Measured: 2 chunks of
+// The floor is the tensor cores' (4 D operations a score). What sets the step is a row tile's chain of
+// scores, softmax, PV and the next scores, which the other tile fills in part: tensor pipe 46%, issue
+// slots 49% and exponentials 47% busy, none of them full. Longer chains cost at once: an eighth of the
+// exponentials on the FMA pipe made it 5% slower. Measured: 2 chunks of
 // 512 tokens over 16384 keys, 32 heads of 128 over 8, 271 GFLOP, 287 us (943 TFLOP/s, 0.57 of the
 // bf16 peak); a step of 256 rows and 128 keys takes 2.35 us, a piece of work 10 us beside its steps.
 //
