@@ -293,6 +293,22 @@ struct Pieces {
   }
 };
 
+// The pieces of a share for warps that meet at a barrier without a time limit, which each of them runs:
+// next() is 1 where a piece came, 0 after the last one, -1 where the wait for it ran out; agree(ok) is
+// the barrier, the same in every warp: whether all are ok; work() does a piece and ends as agree()
+// ended last. A warp that gave up still comes to the barrier, once, and all leave together: none
+// waits there for one that has left.
+#pragma nv_exec_check_disable
+template <typename Next, typename Agree, typename Work>
+__host__ __device__ __forceinline__ bool pieces_together(Next next, Agree agree, Work work) {
+  while (true) {
+    const int got = next();
+    if (!agree(got >= 0)) return false;
+    if (got == 0) return true;
+    if (!work()) return false;
+  }
+}
+
 // A later kernel of the stream may start before this one ends (it waits for its results itself).
 __device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

@@ -368,7 +368,8 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
     const uint32_t part = (static_cast<uint32_t>(v_piece) * 2) ^ static_cast<uint32_t>(v_row & 7);
     int base = 0;
     Piece o{};
-    while (ok && next_piece(o)) {
+    auto next = [&]() -> int { return next_piece(o) ? 1 : ok ? 0 : -1; };
+    ok = pieces_together(next, conv_sync, [&]() -> bool {
       const int k0 = o.t0 * 128;
       const int* bt = a.bt + o.b * a.bt_stride;
       // Key tid of a tile: its page (-1: no key, -2: refused), then its scales.
@@ -418,8 +419,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
         page = page_for(n + 2);
         const bool go = wait_warp(CB_RF + u % C::RAW, static_cast<uint32_t>(u / C::RAW) & 1u) &&
                         wait_warp(CB_VE + u % CH_VSLOTS, (static_cast<uint32_t>(u / CH_VSLOTS) & 1u) ^ 1u);
-        ok = conv_sync(go);  // (also: the conversion reads the scales of the others' keys)
-        if (!ok) break;
+        if (!conv_sync(go)) return false;  // (also: the conversion reads the scales of the others' keys)
         const uint8_t* src = smem + C::OFF_RAW + (u % C::RAW) * C::CODES + v_row * 128;
         uint8_t* dst = smem + C::OFF_V + (u % CH_VSLOTS) * C::VTILE + v_row * 128;
         const uint32_t* vsc = entry + 128 + v_row;
@@ -449,7 +449,8 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
         mbar_arrive(bar(CB_VF + u % CH_VSLOTS));
       }
       base += o.tiles;
-    }
+      return true;
+    });
   } else if (warp == CH_MMA_WARP) {
     // -------------------------------------------------------------- products
     fa2::reg_dealloc<CH_REGS_MMA>();
