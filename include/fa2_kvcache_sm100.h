@@ -20,7 +20,9 @@
  * j % page_size. Table entries past a sequence's last page are not read. Device-side reports go
  * to err_flag as in fa2_sm100.h: FA2_ERR_SHAPE (a length that is negative, longer than the table
  * or the declared maximum, or not covered by its tensor) and FA2_ERR_PAGE (a table entry outside
- * the cache); the row or sequence in question is left out, nothing is accessed out of range.
+ * the cache); the row or sequence in question is left out, nothing is accessed out of range. A word
+ * that already holds a report changes nothing here; fa2_fwd_sm100's kernels stop for one in theirs,
+ * so give these calls another word than those.
  */
 #ifndef FA2_KVCACHE_SM100_H_
 #define FA2_KVCACHE_SM100_H_

@@ -79,6 +79,7 @@ struct Ch {
   static constexpr int OFF_PIECE = OFF_QS + 1024;               // [piece] 12 words
   static constexpr int OFF_BAR = OFF_PIECE + CH_PIECES * 48;
   static constexpr int OFF_TMEM = OFF_BAR + 384;
+  static constexpr int OFF_STOP = OFF_TMEM + 8;
   static constexpr int SMEM = OFF_TMEM + 16 + 1024;             // and slack to align the base
   // The merge of two tiles of the same rows: 64 columns of tile 1's O at a time, where its Q would be.
   static constexpr int COLS = D < 64 ? D : 64;
@@ -169,9 +170,13 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
   auto bar = [&](int i) -> uint32_t { return sbase + C::OFF_BAR + 8u * static_cast<uint32_t>(i); };
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
   const long long timeout = a.timeout > 0 ? a.timeout : CH_TIMEOUT;
+  // Not zero once a wait of this CTA has run out: the others' waits end too. (Not the caller's error word:
+  // that one may hold a refused page or length, of this call or an earlier one, which stops nobody.)
+  int* const stop = reinterpret_cast<int*>(smem + C::OFF_STOP);
   allow_next();
 
   if (warp == 0) {
+    if (lane == 0) *stop = 0;
     auto count_of = [&](int i) -> uint32_t {
       if (i < CB_S) return 128;                     // a tile's softmax threads: Q is written
       if (i < CB_P) return 1;                       // products' commits
@@ -202,8 +207,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + C::OFF_TMEM);
   bool ok = true;
 
-  // A waiting warp; the issuing thread alone waits by itself.
-  auto wait_warp = [&](int i, uint32_t parity) -> bool { return mbar_wait_warp(bar(i), parity, timeout, a.err); };
+  auto wait_warp = [&](int i, uint32_t parity) -> bool { return mbar_wait_warp(bar(i), parity, timeout, stop); };
   auto piece_at = [&](int i) -> volatile int* {
     return reinterpret_cast<volatile int*>(smem + C::OFF_PIECE + (i % CH_PIECES) * 48);
   };
@@ -862,7 +866,10 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
     }
   }
 
-  if (!ok) report(a.err, FA2_ERR_TIMEOUT);
+  if (!ok) {
+    *static_cast<volatile int*>(stop) = 1;
+    report(a.err, FA2_ERR_TIMEOUT);
+  }
   tc_fence_before();
   __syncthreads();
   if (warp == CH_MMA_WARP) {

@@ -86,23 +86,25 @@ def should_pack_gqa(n_q, group, block_m):
 
 
 def _err_word(device):
-    """Per-device int32 that the kernel ORs FA2_ERR_TIMEOUT into when a bounded wait expires."""
+    """Per-device int32 words of the kernels' reports: the first one is that of this module's kernels,
+    whose waits end as soon as it is not zero; the second that of fa2.kvcache, whose reports stop no
+    other call."""
     key = device.index
     w = _err_words.get(key)
     if w is None:
-        w = torch.zeros(1, dtype=torch.int32, device=device)
+        w = torch.zeros(2, dtype=torch.int32, device=device)
         _err_words[key] = w
     return w
 
 
 def check_device_errors(device=None):
-    """Synchronise `device` and raise RuntimeError if a kernel reported a timed-out wait
-    since the last check (the word is cleared). Launches never synchronise on their own."""
+    """Synchronise `device` and raise RuntimeError if a kernel reported a timed-out wait or refused a
+    length or page since the last check (the words are cleared). Launches never synchronise on their own."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     w = _err_words.get(device.index)
     if w is None:
         return
-    val = int(w.item())
+    val = next((v for v in w.tolist() if v), 0)
     if val:
         w.zero_()
         raise RuntimeError(f"fa2 sm100 kernel reported status {val}: {_lib.strerror(val)}")

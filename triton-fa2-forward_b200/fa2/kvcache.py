@@ -110,6 +110,12 @@ def _table(block_table):
     return block_table if block_table.stride(1) == 1 or block_table.shape[1] <= 1 else block_table.contiguous()
 
 
+def _report_word(device):
+    """Address of the device's error word of these kernels: not the one of fa2.kernel's, which stop for
+    any report in theirs."""
+    return _err_word(device).data_ptr() + 4
+
+
 def _launch(entry, packed, index):
     _kvlib.launch(entry, packed, index)
     if _sync_check_enabled():
@@ -148,7 +154,7 @@ def kvcache_append_fp8(k, v, cache, block_table, cache_seqlens, cu_seqlens=None)
     bt, sl = _table(block_table), cache_seqlens.contiguous()
     packed = _kvlib.APPEND.pack(
         *fields, k.data_ptr(), v.data_ptr(), *_rows(k), *_rows(v), bt.data_ptr(), sl.data_ptr(), cu,
-        _err_word(k.device).data_ptr(), bt.stride(0), bt.shape[1], B, n, dtype == torch.bfloat16)
+        _report_word(k.device), bt.stride(0), bt.shape[1], B, n, dtype == torch.bfloat16)
     _launch(_kvlib.lib().fa2_kv8_append_sm100, packed, index)
     return cache
 
@@ -171,7 +177,7 @@ def kvcache_read_fp8(cache, block_table, cu_seqlens, total, dtype=torch.bfloat16
         return k, v
     bt, cu = _table(block_table), cu_seqlens.contiguous()
     packed = _kvlib.READ.pack(
-        *fields, k.data_ptr(), v.data_ptr(), bt.data_ptr(), cu.data_ptr(), _err_word(device).data_ptr(),
+        *fields, k.data_ptr(), v.data_ptr(), bt.data_ptr(), cu.data_ptr(), _report_word(device),
         bt.stride(0), bt.shape[1], B, total, dtype == torch.bfloat16)
     _launch(_kvlib.lib().fa2_kv8_read_sm100, packed, index)
     return k, v
@@ -233,7 +239,7 @@ def attention_kvcache_fp8(q, cache, block_table, cache_seqlens, max_seqlen_k=Non
         oo = torch.empty_like(qq)
     L = _kvlib.lib()
     head = (*fields, qq.data_ptr(), oo.data_ptr(), *_rows(qq), *_rows(oo), bt.data_ptr(), sl.data_ptr(),
-            cu_seqlens_q.data_ptr() if packed else 0, _err_word(q.device).data_ptr())
+            cu_seqlens_q.data_ptr() if packed else 0, _report_word(q.device))
     tail = (bt.stride(0), 0, pages_per_seq, B, H_q, n_q, q_shape[0] if packed else 0, int(max_seqlen_k),
             dtype == torch.bfloat16, bool(causal), CAUSAL_ALIGNS[causal_align],
             0 if num_splits is None else max(1, int(num_splits)), sm_scale * LOG2E, 0)
