@@ -26,3 +26,9 @@ def run_program(tmp_path_factory):
 def test_converting_warps_leave_together(run_program):
     """A warp that gives up at the wait for a piece or inside one leaves no other at their barrier."""
     run_program("pieces_together")
+
+
+def test_line_of_work(run_program):
+    """Shares of valid calls cover every tile once, cuts are where the merge looks; sums of query lengths that
+    go back and forth, up to sums past 32 bits, lead nowhere outside the tensors."""
+    run_program("line")

@@ -41,20 +41,20 @@ constexpr float RESCALE_TH = 8.0f;  // log2: the reference max moves when a row'
 constexpr int P_SHIFT = 6;          // P' = p * sv * 2^(P_SHIFT - e), see above
 constexpr int EB_MIN = 8;           // smallest exponent field used for e (a multiplier stays finite)
 
-__device__ __forceinline__ int query_of(const AttnArgs& a, int row) { return divide(a.by_group, row); }
+FA2_HOST_DEVICE int query_of(const AttnArgs& a, int row) { return divide(a.by_group, row); }
 
 struct Seq {
   int n_q, q0, len, off;  // queries, first packed row, keys, causal offset
 };
 
 // Sequence b, checked: nothing its numbers lead to is outside the tensors.
-__device__ __forceinline__ Seq sequence(const AttnArgs& a, int b) {
+FA2_HOST_DEVICE Seq sequence(const AttnArgs& a, int b) {
   Seq s;
   s.n_q = a.n_q;
   s.q0 = 0;
   if (a.cu_q != nullptr) {
-    s.q0 = __ldg(a.cu_q + b);
-    const int64_t end = __ldg(a.cu_q + b + 1);
+    s.q0 = load_int(a.cu_q + b);
+    const int64_t end = load_int(a.cu_q + b + 1);
     const int64_t n = end - s.q0;
     if (s.q0 < 0 || n < 0 || n > a.n_q || end > a.total_q) {
       report(a.err, FA2_ERR_SHAPE);
@@ -63,7 +63,7 @@ __device__ __forceinline__ Seq sequence(const AttnArgs& a, int b) {
       s.n_q = static_cast<int>(n);
     }
   }
-  s.len = __ldg(a.lens + b);
+  s.len = load_int(a.lens + b);
   if (s.len < 0 || s.len > a.max_k || s.len > static_cast<int64_t>(a.pages_per_seq) * a.c.page_size) {
     report(a.err, FA2_ERR_SHAPE);
     s.len = 0;
@@ -73,7 +73,7 @@ __device__ __forceinline__ Seq sequence(const AttnArgs& a, int b) {
 }
 
 // Keys that the rows [row0, row0 + count) of a (sequence, kv head) see at most: [0, result).
-__device__ __forceinline__ int keys_end(const AttnArgs& a, const Seq& s, int row0, int count) {
+FA2_HOST_DEVICE int keys_end(const AttnArgs& a, const Seq& s, int row0, int count) {
   if (!a.causal) return s.len;
   const int i = min(query_of(a, row0 + count - 1), s.n_q - 1);
   return max(0, min(s.len, i + s.off + 1));
@@ -117,16 +117,16 @@ struct Cut {
 // the shares are long enough for that to matter.
 struct Line {
   // Tiles and tile cost of row block rb of sequence s, and the sum over a sequence's blocks.
-  __device__ static int blocks(const AttnArgs& a, const Seq& s) { return (s.n_q * a.group + a.block - 1) / a.block; }
-  __device__ static int tiles(const AttnArgs& a, const Seq& s, int rb) {
+  FA2_HOST_DEVICE static int blocks(const AttnArgs& a, const Seq& s) { return (s.n_q * a.group + a.block - 1) / a.block; }
+  FA2_HOST_DEVICE static int tiles(const AttnArgs& a, const Seq& s, int rb) {
     const int rows = s.n_q * a.group, row0 = rb * a.block;
     return (keys_end(a, s, row0, min(a.block, rows - row0)) + 127) / 128;
   }
-  __device__ static int tile_cost(const AttnArgs& a, const Seq& s, int rb) {
+  FA2_HOST_DEVICE static int tile_cost(const AttnArgs& a, const Seq& s, int rb) {
     return a.block < 256 ? 1 : s.n_q * a.group - rb * 256 > 128 ? 4 : 3;
   }
   // A kv head's tiles (cost) and blocks that have any.
-  __device__ static void head_cost(const AttnArgs& a, const Seq& s, int& tiles_cost, int& n_blocks) {
+  FA2_HOST_DEVICE static void head_cost(const AttnArgs& a, const Seq& s, int& tiles_cost, int& n_blocks) {
     tiles_cost = n_blocks = 0;
     for (int rb = 0; rb < blocks(a, s); ++rb) {
       const int n = tiles(a, s, rb);
@@ -137,16 +137,16 @@ struct Line {
   // From the tiles' cost: the workers that get something, and a block's own cost. Every share is at
   // least as long as a block's own cost and a tile, so one that begins or ends inside a block but for
   // its first tile holds one of its tiles.
-  __device__ static int workers(const AttnArgs& a, int cost) { return min(a.workers, a.block < 256 ? cost : max(1, cost / 4)); }
-  __device__ static int block_cost(const AttnArgs& a, int cost) {
+  FA2_HOST_DEVICE static int workers(const AttnArgs& a, int cost) { return min(a.workers, a.block < 256 ? cost : max(1, cost / 4)); }
+  FA2_HOST_DEVICE static int block_cost(const AttnArgs& a, int cost) {
     return a.block < 256 ? 0 : min(16, max(0, cost / a.workers - 4));
   }
   // Where worker w's share starts, and the worker whose share holds position x.
-  __device__ static int start(int w, int workers, int total) {  // w total / workers, in 32 bits
+  FA2_HOST_DEVICE static int start(int w, int workers, int total) {  // w total / workers, in 32 bits
     const uint32_t q = static_cast<uint32_t>(total) / static_cast<uint32_t>(workers), r = total - q * workers;
     return static_cast<int>(w * q + w * r / static_cast<uint32_t>(workers));  // (w r < workers^2)
   }
-  __device__ static int holder(int x, int workers, int total) {
+  FA2_HOST_DEVICE static int holder(int x, int workers, int total) {
     int w = min(workers - 1, static_cast<int>((x + 0.5f) * workers / total));  // off by one at most
     while (w > 0 && start(w, workers, total) > x) --w;
     while (w + 1 < workers && start(w + 1, workers, total) <= x) ++w;
@@ -154,54 +154,75 @@ struct Line {
   }
 };
 
-// Finds, with a warp, the length of the line, this worker's share of it and a sequence at or before
-// the share's start. Each lane adds up a run of sequences.
+// A worker's share of the line and a sequence at or before its start.
 struct Share {
   int total, workers, block_cost;
   int p0, p1;         // this worker's share
   int b, start_b;     // the first sequence of the run that holds p0, and where it starts
 };
-// A line whose cost reaches LONGEST_LINE is refused and nothing is done. The host's limits keep every line
-// of sequences that do not overlap below it; sums of query lengths that go back and forth could
-// count the same queries many times.
+// A line of LONGEST_LINE cost units or more is refused and nothing is done. The host's limits keep every
+// line of sequences that do not overlap below it; sums of query lengths that go back and forth could
+// count the same queries many times. Positions are 32 bits, so the sums over the line stop there.
 constexpr int LONGEST_LINE = (1 << 30) - 1;
-__device__ __forceinline__ Share find_share(const AttnArgs& a, int w) {
-  const int lane = static_cast<int>(threadIdx.x) & 31, per = (a.batch + 31) / 32;
-  const int b0 = min(a.batch, lane * per), b1 = min(a.batch, b0 + per);
-  int own = 0, own_blocks = 0;
+FA2_HOST_DEVICE int line_sum(int x, int y) { return x + y < LONGEST_LINE ? x + y : LONGEST_LINE; }
+
+// Tiles' cost and blocks of a run of sequences.
+struct Run {
+  int b0, cost, blocks;
+};
+// Those of lane `lane`, one of the 32 runs that the sequences are divided into. (A sequence alone is below
+// 2^29: the host's limits hold for each.)
+FA2_HOST_DEVICE Run run_of(const AttnArgs& a, int lane) {
+  const int per = (a.batch + 31) / 32, first = lane * per;
+  Run r{first < a.batch ? first : a.batch, 0, 0};
+  const int end = r.b0 + per < a.batch ? r.b0 + per : a.batch;
 #pragma unroll 1
-  for (int b = b0; b < b1; ++b) {
+  for (int b = r.b0; b < end; ++b) {
     int cost, n;
     Line::head_cost(a, sequence(a, b), cost, n);
-    own = min(LONGEST_LINE, own + a.heads_kv * cost);
-    own_blocks = min(LONGEST_LINE, own_blocks + a.heads_kv * n);
+    r.cost = line_sum(r.cost, a.heads_kv * cost);
+    r.blocks = line_sum(r.blocks, a.heads_kv * n);
   }
-  int sum = own, sum_blocks = own_blocks;
+  return r;
+}
+// Worker w's share of a line of tiles that cost `cost` in `blocks` blocks; false where it is refused.
+FA2_HOST_DEVICE bool share_of(const AttnArgs& a, int w, int cost, int blocks, Share& r) {
+  r = Share{};
+  const int block_cost = Line::block_cost(a, cost);
+  const int64_t total = cost + static_cast<int64_t>(block_cost) * blocks;  // (blocks <= cost)
+  if (total >= LONGEST_LINE) return false;
+  r.workers = Line::workers(a, cost);
+  r.block_cost = block_cost;
+  r.total = static_cast<int>(total);
+  if (w < r.workers) {
+    r.p0 = Line::start(w, r.workers, r.total);
+    r.p1 = Line::start(w + 1, r.workers, r.total);
+  }
+  return true;
+}
+
+// Finds a worker's share with a warp: each lane adds up a run.
+__device__ __forceinline__ Share find_share(const AttnArgs& a, int w) {
+  const int lane = static_cast<int>(threadIdx.x) & 31;
+  const Run run = run_of(a, lane);
+  int sum = run.cost, sum_blocks = run.blocks;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int v = __shfl_up_sync(0xffffffffu, sum, o), n = __shfl_up_sync(0xffffffffu, sum_blocks, o);
     if (lane >= o) {
-      sum = min(LONGEST_LINE, sum + v);
-      sum_blocks = min(LONGEST_LINE, sum_blocks + n);
+      sum = line_sum(sum, v);
+      sum_blocks = line_sum(sum_blocks, n);
     }
   }
   Share r;
-  const int cost = __shfl_sync(0xffffffffu, sum, 31);
-  if (cost >= LONGEST_LINE) {
+  if (!share_of(a, w, __shfl_sync(0xffffffffu, sum, 31), __shfl_sync(0xffffffffu, sum_blocks, 31), r)) {
     report(a.err, FA2_ERR_SHAPE);
-    r = Share{};
     return r;
   }
-  r.workers = Line::workers(a, cost);
-  r.block_cost = Line::block_cost(a, cost);
-  r.total = cost + r.block_cost * __shfl_sync(0xffffffffu, sum_blocks, 31);
-  r.p0 = w < r.workers ? Line::start(w, r.workers, r.total) : 0;
-  r.p1 = w < r.workers ? Line::start(w + 1, r.workers, r.total) : 0;
-  own += r.block_cost * own_blocks;
-  const int before = sum + r.block_cost * sum_blocks - own;
+  const int own = run.cost + r.block_cost * run.blocks, before = sum + r.block_cost * sum_blocks - own;
   const uint32_t at = __ballot_sync(0xffffffffu, before <= r.p0 && r.p0 < before + own);
   const int from = at != 0 ? __ffs(at) - 1 : 0;
-  r.b = __shfl_sync(0xffffffffu, b0, from);
+  r.b = __shfl_sync(0xffffffffu, run.b0, from);
   r.start_b = __shfl_sync(0xffffffffu, before, from);
   return r;
 }
@@ -214,10 +235,10 @@ struct Block {
   int first;            // position of the block
   // The first tile at or behind position p. A share that begins or ends inside a tile: the tile
   // belongs to the earlier worker.
-  __device__ int tile_of(int p) const { return p <= at ? 0 : min(tiles, (p - at + cost - 1) / cost); }
+  FA2_HOST_DEVICE int tile_of(int p) const { return p <= at ? 0 : min(tiles, (p - at + cost - 1) / cost); }
 };
 // The block that holds position p, walking on from sequence b, which starts at `start`.
-__device__ __forceinline__ void find_block(const AttnArgs& a, int block_cost, int p, int& b, int& start, Block& o) {
+FA2_HOST_DEVICE void find_block(const AttnArgs& a, int block_cost, int p, int& b, int& start, Block& o) {
   int hc;
   while (true) {
     o.sq = sequence(a, b);
@@ -258,7 +279,7 @@ struct Pieces {
     w = worker;
     if (s.p0 >= s.p1) a.cuts[w].n_parts = 0;
   }
-  __device__ bool next(const AttnArgs& a, Piece& o) {
+  FA2_HOST_DEVICE bool next(const AttnArgs& a, Piece& o) {
     while (p < s.p1) {
       Block k;
       find_block(a, s.block_cost, p, s.b, s.start_b, k);

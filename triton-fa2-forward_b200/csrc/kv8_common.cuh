@@ -28,12 +28,27 @@ struct Cache {
   int k_page16, v_page16, ks_page, vs_page, k_row, v_row, ks_row, vs_row, k_head, v_head, ks_head, vs_head;
 };
 
+// What the tests run on the host as well: reads and reports in both forms.
+#define FA2_HOST_DEVICE __host__ __device__ __forceinline__
+FA2_HOST_DEVICE int load_int(const int* p) {
+#ifdef __CUDA_ARCH__
+  return __ldg(p);
+#else
+  return *p;
+#endif
+}
+
 __device__ __forceinline__ int page_of(const Cache& c, int pos) {
   return c.page_shift >= 0 ? pos >> c.page_shift : pos / c.page_size;
 }
 
-__device__ __forceinline__ void report(int* err, int code) {
-  if (err != nullptr) atomicCAS(err, 0, code);  // the first report wins
+FA2_HOST_DEVICE void report(int* err, int code) {
+  if (err == nullptr) return;
+#ifdef __CUDA_ARCH__
+  atomicCAS(err, 0, code);  // the first report wins
+#else
+  if (*err == 0) *err = code;
+#endif
 }
 
 // Two values to two e4m3 codes (low byte: lo), round to nearest even, saturated at +-448.
@@ -116,8 +131,13 @@ struct Divisor {
   uint32_t mul;
   int shift;
 };
-__device__ __forceinline__ int divide(const Divisor& v, int n) {
-  return v.d == 1 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), v.mul) >> v.shift);
+FA2_HOST_DEVICE int divide(const Divisor& v, int n) {
+#ifdef __CUDA_ARCH__
+  const uint32_t hi = __umulhi(static_cast<uint32_t>(n), v.mul);
+#else
+  const uint32_t hi = static_cast<uint32_t>(static_cast<uint64_t>(static_cast<uint32_t>(n)) * v.mul >> 32);
+#endif
+  return v.d == 1 ? n : static_cast<int>(hi >> v.shift);
 }
 
 // ------------------------------------------------------------------------------------ host
