@@ -125,10 +125,12 @@ typedef struct Fa2Kv8ReadParams {
 
 /* out = softmax(q k^T * sm_scale + mask) v over the cache. q, o: [B, H_q, N, D], or packed
  * [total, H_q, D] with cu_seqlens_q (the token axis as n). causal_align as in fa2_sm100.h, per
- * sequence. A query that sees no key gets zeros, and so does a sequence whose length is refused. The
- * sequences of a call share the GPU as one line of work that is cut into equal shares, and partial sums
- * are joined in its order: the same call gives the same bits, but another batch around a sequence may
- * cut it elsewhere and change its last bits. */
+ * sequence. A query that sees no key gets zeros, and so do those of a sequence whose cache_seqlens entry is
+ * refused. Not written: rows of no sequence; rows of one whose number of queries is refused (negative, above
+ * seqlen_q, or past total_q); every row that sees a key, where sums that go back and forth make 2^30 units
+ * of work or more (FA2_ERR_SHAPE). The sequences of a call share the GPU as one line of work that is cut into
+ * equal shares, and partial sums are joined in its order: the same call gives the same bits, but another batch
+ * around a sequence may cut it elsewhere and change its last bits. */
 typedef struct Fa2Kv8AttnParams {
   Fa2Kv8Cache cache;
   const void* q;

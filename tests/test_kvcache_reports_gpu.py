@@ -92,3 +92,21 @@ def test_a_limit_of_one_clock_ends_the_call(dtype, N_q, monkeypatch):
             assert f"status {_lib.FA2_ERR_TIMEOUT}:" in str(e)
     monkeypatch.undo()
     assert torch.equal(attention_kvcache_fp8(q, cache, bt, sl), good)
+
+
+@pytest.mark.parametrize("group,N_q", [(2, 6), (8, 40)])
+def test_a_refused_number_of_queries_leaves_the_others_alone(group, N_q):
+    """Sums that fall, leave q or exceed the declared maximum."""
+    cache, bt, sl, _, _, _ = filled([300, 200, 150], 64, 2, 64, seed=27)
+    q = randn(3 * N_q + 3, 2 * group, 64, dtype=torch.bfloat16, seed=28)
+    total = q.shape[0]
+    for cu, good in (([0, N_q, 2 * N_q + 1, 3 * N_q], [0, 2]), ([0, N_q, N_q - 3, N_q - 3], [0]),
+                     ([0, N_q, 2 * N_q, total + 1], [0, 1])):
+        cu_t = torch.tensor(cu, dtype=torch.int32).cuda()
+        out = attention_kvcache_fp8(q, cache, bt, sl, cu_seqlens_q=cu_t, max_seqlen_q=N_q)
+        reported(_lib.FA2_ERR_SHAPE)
+        for b in good:
+            alone = torch.tensor([0, cu[b + 1] - cu[b]], dtype=torch.int32).cuda()
+            ref, weight, spread, small = serving.attention(q[cu[b]:cu[b + 1]], cache, bt[b:b + 1], sl[b:b + 1], cu_seqlens_q=alone)
+            got, qs = out[cu[b]:cu[b + 1]], q[cu[b]:cu[b + 1]]
+            assert ((got.double() - ref).abs() <= tolerance(qs, weight, spread, small, ref, 300, 8.0)).all()

@@ -195,8 +195,9 @@ def attention_kvcache_fp8(q, cache, block_table, cache_seqlens, max_seqlen_k=Non
     last positions). A query that sees no key gets zeros, one that sees a key of a refused page NaN.
     num_splits: CTAs that share the work for each (sequence, kv head, block of rows); None: chosen from
     the sizes. The same call gives the same bits; another batch around a sequence may cut its keys
-    elsewhere and change its last bits. Returns a tensor like q (rows past cu_seqlens_q[B] are not
-    written), asynchronously.
+    elsewhere and change its last bits. Returns a tensor like q, asynchronously. Not written are rows past
+    cu_seqlens_q[B] and, beside a device error, those of a sequence whose sums fall, leave q or give more
+    than max_seqlen_q queries (all rows, where sums go back and forth thousands of times).
     """
     fields, shape, tensors = _cache_fields(cache)
     q_shape, dtype = q.shape, q.dtype
