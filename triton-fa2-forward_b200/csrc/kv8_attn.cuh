@@ -3,8 +3,8 @@
 // With codes c and row scales s, and q scaled by a power of two f_i:
 //     x_ij = sm_scale * log2(e) / f_i * (sum_d q'_id ck_jd) * sk_j      p_ij = 2^(x_ij - m_i)
 //     o_i  = sum_j (p_ij sv_j) cv_j / sum_j p_ij
-// The first product runs on fp16 operands for few rows (q' below 2^15, exact) and on e4m3 operands
-// for many (see there). The second runs on fp16: e4m3 codes are exact in it, and P' = p_ij sv_j
+// The first product runs on fp16 operands for few rows (q' below 2^15, exact) and on 8-bit ones for
+// many (see there). The second runs on fp16: e4m3 codes are exact in it, and P' = p_ij sv_j
 // 2^(6 - e), with e the largest exponent of the sv seen so far, is rounded to it (relative error
 // 2^-11, below half a step of the output; P' < 2^15, and its range reaches 2^-30 below the row's
 // largest p). Sums, statistics and scales are fp32.

@@ -13,11 +13,15 @@
 // the work (see Line); the rings and barriers carry over from one piece to the next.
 //
 // QK^T runs on the codes as they are stored: K is an e4m3 operand, and a row of Q, times the power
-// of two that brings its largest value into [128, 256), is the sum of two e4m3 operands for bf16
-// (8 significant bits: 4 and a sign's 4) or three for fp16 (11 bits). That is exact but for values
-// more than 2^10 below the row's largest, which are off by at most 2^-17 of it. 8-bit products run
-// at twice the rate of 16-bit ones, so the second operand costs nothing over converting K to fp16
-// (64 instructions less for each 16 values).
+// of two that brings its largest value into [128, 256), is the sum of an e4m3 operand and one (bf16) or
+// two (fp16) e5m2 operands, each the rounding of what the ones before leave. From 2^-6 on the first one has
+// 4 significant bits and leaves at most 8 units of the last place of a bf16 value, or 64 of an fp16 value:
+// whole numbers up to 8 have 3 significant bits, as e5m2 has, and of those up to 64 a second e5m2 term takes
+// the at most 4 units that the first leaves. So every value within 2^13 of its row's largest is exact.
+// A smaller one is off by at most 2^-14 (bf16) or 2^-17 (fp16: half of e5m2's smallest step), which is
+// 2^-21 or 2^-24 of the largest. (With e4m3 for all terms, whose smallest step is 2^-9, exactness ended
+// 2^6 to 2^10 below the largest.) 8-bit products run at twice the rate of 16-bit ones, so the second
+// operand costs nothing over converting K to fp16 (64 instructions less for each 16 values).
 //
 // PV runs on fp16: P' needs 11 bits. V is converted on its way into shared memory. Its row scales:
 // bf16 queries fold them into that conversion (code * s_j in fp16, one rounding of at most 2^-11, an
@@ -59,7 +63,7 @@ constexpr int FOLD_SHIFT = 6;   // folded scales: the largest lies in [2^6, 2^7)
 
 template <int D, bool BF16>
 struct Ch {
-  static constexpr int TERMS = BF16 ? 2 : 3;          // e4m3 operands of Q
+  static constexpr int TERMS = BF16 ? 2 : 3;          // operands of Q: e4m3, then e5m2
   static constexpr int KSLOTS = BF16 ? 3 : 2;         // rings of K codes ...
   static constexpr int RAW = BF16 ? 2 : 1;            // ... and V codes
   static constexpr int KSTEPS = D > 32 ? D / 32 : 1;  // 32-wide steps of QK^T (D = 16: zeros beyond)
@@ -101,8 +105,8 @@ __device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) { retur
 // The issuing warp runs converged and its lane 0 issues (`lead`, a predicate and no branch): the
 // descriptors stay in uniform registers, which the products take. Issued inside a branch of one lane
 // every operand is moved there first, and a step of the loop took 1.3 to 2 times as long.
-// D[tmem] (+)= A[smem] * B[smem], both e4m3 (32 wide steps), fp32 sums. Operands: lower descriptor words.
-__device__ __forceinline__ void mma_e4m3(uint32_t lead, uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t add) {
+// D[tmem] (+)= A[smem] * B[smem], 8-bit floats by `idesc` (32 wide steps), fp32 sums. Operands: lower descriptor words.
+__device__ __forceinline__ void mma_f8(uint32_t lead, uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t add) {
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
       "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
@@ -125,9 +129,10 @@ __device__ __forceinline__ void commit_to(uint32_t lead, uint32_t bar) {
       "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(lead)
       : "memory");
 }
-// Instruction descriptor of kind::f8f6f4: fp32 D, e4m3 A and B (type codes 0), both K-major.
-__host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N) {
-  return (1u << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+// Instruction descriptor of kind::f8f6f4: fp32 D, A in e4m3 (type code 0) or e5m2 (1), B in e4m3, both
+// K-major.
+__host__ __device__ constexpr uint32_t idesc_f8(int M, int N, bool a_e5m2) {
+  return (1u << 4) | (a_e5m2 ? 1u << 7 : 0u) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
 
 __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
@@ -458,7 +463,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
   } else if (warp == CH_MMA_WARP) {
     // -------------------------------------------------------------- products
     fa2::reg_dealloc<CH_REGS_MMA>();
-    constexpr uint32_t idesc_qk = idesc_e4m3(128, 128);
+    constexpr uint32_t idesc_qk = idesc_f8(128, 128, false), idesc_qk5 = idesc_f8(128, 128, true);
     constexpr uint32_t idesc_pv = fa2::idesc_f16(false, 128, D, true);
     const uint32_t dq = desc_lo(sbase + C::OFF_Q, 16), dk = desc_lo(sbase + C::OFF_K, 16);
     const uint32_t dv = desc_lo(sbase + C::OFF_V, C::CHUNK);
@@ -511,7 +516,8 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
 #pragma unroll
           for (int i = 0; i < C::TERMS * C::KSTEPS; ++i) {
             const uint32_t kk = static_cast<uint32_t>(i % C::KSTEPS), term = static_cast<uint32_t>(i / C::KSTEPS);
-            mma_e4m3(lead, tmem + t * 128, qd + (term * C::CODES + kk * 32) / 16, kd + kk * 2, idesc_qk, i > 0 ? 1u : 0u);
+            mma_f8(lead, tmem + t * 128, qd + (term * C::CODES + kk * 32) / 16, kd + kk * 2, term == 0 ? idesc_qk : idesc_qk5,
+                   i > 0 ? 1u : 0u);
           }
           commit_to(lead, bar(CB_S + t));
           if (last_use) commit_to(lead, bar(CB_KE + u % C::KSLOTS));
@@ -538,7 +544,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
       const int rows = o.sq.n_q * a.group, row0 = o.rb * 256, k0 = o.t0 * 128;
       const bool dual = rows - row0 <= 128;
       const int tile_row0 = row0 + (dual ? 0 : t * 128), row = tile_row0 + r;
-      // Q: a warp's 32 rows as e4m3 terms, 8 lanes (D / 16) a row, 16 values each; every row times the power
+      // Q: a warp's 32 rows as 8-bit terms, 8 lanes (D / 16) a row, 16 values each; every row times the power
       // of two that brings its largest value into [128, 256). Each term is the rounding of what the
       // terms before leave (an exact difference in fp32). The raw values come by asynchronous copies, all
       // under way at once, to where this lane's first two terms go: it alone reads and overwrites them.
@@ -593,9 +599,11 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
               uint32_t y[4];
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
-                const uint16_t lo = e4m3x2(x[4 * j], x[4 * j + 1]), hi = e4m3x2(x[4 * j + 2], x[4 * j + 3]);
+                const uint16_t lo = term == 0 ? e4m3x2(x[4 * j], x[4 * j + 1]) : e5m2x2(x[4 * j], x[4 * j + 1]);
+                const uint16_t hi = term == 0 ? e4m3x2(x[4 * j + 2], x[4 * j + 3]) : e5m2x2(x[4 * j + 2], x[4 * j + 3]);
                 if (term + 1 < C::TERMS) {
-                  const float2 y0 = float2_of_f16x2(f16x2_of_e4m3x2(lo)), y1 = float2_of_f16x2(f16x2_of_e4m3x2(hi));
+                  const float2 y0 = float2_of_f16x2(term == 0 ? f16x2_of_e4m3x2(lo) : f16x2_of_e5m2x2(lo));
+                  const float2 y1 = float2_of_f16x2(term == 0 ? f16x2_of_e4m3x2(hi) : f16x2_of_e5m2x2(hi));
                   x[4 * j] -= y0.x;
                   x[4 * j + 1] -= y0.y;
                   x[4 * j + 2] -= y1.x;

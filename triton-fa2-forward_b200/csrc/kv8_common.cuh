@@ -58,6 +58,20 @@ __device__ __forceinline__ uint16_t e4m3x2(float lo, float hi) {
   return r;
 }
 
+// The same with e5m2 (5 exponent bits, 2 mantissa bits: smallest step 2^-16, saturated at +-57344).
+__device__ __forceinline__ uint16_t e5m2x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Two e5m2 codes to fp16 (exact: e5m2 is its upper byte).
+__device__ __forceinline__ uint32_t f16x2_of_e5m2x2(uint16_t c) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e5m2x2 %0, %1;" : "=r"(r) : "h"(c));
+  return r;
+}
+
 // Two e4m3 codes to fp16 (exact: fp16 holds every e4m3 value).
 __device__ __forceinline__ uint32_t f16x2_of_e4m3x2(uint16_t c) {
   uint32_t r;

@@ -193,6 +193,8 @@ def attention_kvcache_fp8(q, cache, block_table, cache_seqlens, max_seqlen_k=Non
     max_seqlen_k (default: pages_per_seq * page_size; a longer one is reported as a device error and
     attends to nothing). The causal mask is per sequence, bottom-right by default (the queries are the
     last positions). A query that sees no key gets zeros, one that sees a key of a refused page NaN.
+    With more than 16 rows (queries x heads of a group) a query's values are exact within 2^13 of the
+    largest of its row; smaller ones are off by at most 2^-21 (bf16) or 2^-24 (fp16) of that one.
     num_splits: CTAs that share the work for each (sequence, kv head, block of rows); None: chosen from
     the sizes. The same call gives the same bits; another batch around a sequence may cut its keys
     elsewhere and change its last bits. Returns a tensor like q, asynchronously. Not written are rows past
