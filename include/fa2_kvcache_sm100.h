@@ -57,7 +57,8 @@ typedef struct Fa2Kv8Cache {
  *     a' = magnitude * (a cos t - c sin t),  c' = magnitude * (a sin t + c cos t)
  * with -t in place of t when `inverse` (the transposed map: the gradient of the forward one).
  * Pairs are (i, i + rotary_dim / 2), or (2 i, 2 i + 1) when `interleaved`; values from rotary_dim
- * on are copied. out may be in (each value is read before it is written, by the same thread). */
+ * on are copied. out may be in (each value is read before it is written, by the same thread), as long as
+ * every value of q and k has memory of its own. */
 typedef struct Fa2RotaryParams {
   const void* q;
   const void* k;

@@ -7,6 +7,7 @@ Forward only, like attention(): `inverse=True` applies the transposed map, which
 the forward one.
 """
 
+import functools
 import math
 
 import torch
@@ -61,8 +62,55 @@ def _strides4(t):
     return st if len(st) == 4 else (0, st[1], st[0], st[2])  # [total, H, D]
 
 
-def _overlaps(t):
-    return any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride()))
+def _reaches(terms, target, left):
+    """Whether whole numbers lo <= x <= hi exist for the terms (stride, lo, hi) with sum stride * x = target.
+    Largest strides first: as long as a stride is longer than what the smaller ones span, at most two x
+    each are in question. left: [steps], after which the answer is True."""
+    if not terms:
+        return target == 0
+    left[0] -= 1
+    if left[0] < 0:
+        return True
+    (stride, lo, hi), rest = terms[0], terms[1:]
+    least, most = sum(s * a for s, a, _ in rest), sum(s * b for s, _, b in rest)
+    first, last = max(lo, -((most - target) // stride)), min(hi, (target - least) // stride)
+    return any(_reaches(rest, target - stride * x, left) for x in range(first, last + 1))
+
+
+@functools.lru_cache(maxsize=4096)
+def _share_memory(dims, other=None, distance=0):
+    """Whether two values of a tensor of dims ((size, stride), ...) share an address; with the dims of
+    another tensor that starts `distance` elements behind it: a value of each. (Layouts that are too tangled to
+    tell count as sharing.)"""
+    left = [10000]
+    if other is None:
+        dims = sorted(((s, n) for n, s in dims if n > 1), reverse=True)
+        if any(s == 0 for s, _ in dims):
+            return True
+        # The first index that differs is larger in one of the two values by 1 or more.
+        return any(_reaches([(s, 1, n - 1)] + [(t, 1 - m, m - 1) for t, m in dims[i + 1:]], 0, left) for i, (s, n) in enumerate(dims))
+    spans = {}
+    for n, s in dims:
+        if n > 1 and s:
+            lo, hi = spans.get(s, (0, 0))
+            spans[s] = lo, hi + n - 1
+    for n, s in other:
+        if n > 1 and s:
+            lo, hi = spans.get(s, (0, 0))
+            spans[s] = lo - (n - 1), hi
+    return _reaches(sorted(((s, lo, hi) for s, (lo, hi) in spans.items()), reverse=True), distance, left)
+
+
+def _refuse_shared(q, k):
+    """Rotation in place: every value of q and k has memory of its own."""
+    tensors = [t for t in (q, k) if t is not None and t.numel() > 0]
+    dims = [tuple(zip(t.shape, t.stride())) for t in tensors]
+    shared = any(_share_memory(d) for d in dims)
+    if not shared and len(tensors) == 2:
+        shared = _share_memory(dims[0], dims[1], (tensors[1].data_ptr() - tensors[0].data_ptr()) // 2)
+    if shared:
+        raise ValueError("inplace needs tensors whose values do not share memory (no expanded dimensions or overlapping "
+                         "views, no value in both q and k)")
 
 
 def rotary(q, k, positions, inv_freq, interleaved=False, inverse=False, magnitude=1.0, inplace=False):
@@ -75,7 +123,8 @@ def rotary(q, k, positions, inv_freq, interleaved=False, inverse=False, magnitud
     interleaved=True. The angle is formed in 64 bits, so far positions lose nothing.
 
     inverse=True turns by the negative angle: with the same magnitude, the gradient of the forward
-    map. inplace=True writes into q and k themselves. Returns (q', k'); k' is None where k is.
+    map. inplace=True writes into q and k themselves, which may be views of one buffer but have no value
+    in common. Returns (q', k'); k' is None where k is.
     Asynchronous on torch's current stream.
     """
     dims, dtype = q.dim(), q.dtype
@@ -104,6 +153,8 @@ def rotary(q, k, positions, inv_freq, interleaved=False, inverse=False, magnitud
     assert 2 <= rd <= D, "inv_freq must have between 1 and D / 2 entries"
     if not 0 < magnitude < 3e38:
         raise ValueError(f"magnitude must be positive and finite, got {magnitude}")
+    if inplace:
+        _refuse_shared(q, k)
     index = q.get_device()  # -1: not on CUDA
     if index < 0 or positions.get_device() < 0 or inv_freq.get_device() < 0 or (k is not None and k.get_device() < 0):
         raise RuntimeError("fa2.rotary.rotary runs only on an sm_100 CUDA device (no CPU path)")
@@ -115,8 +166,6 @@ def rotary(q, k, positions, inv_freq, interleaved=False, inverse=False, magnitud
     if k is not None and H_kv == 0:
         raise ValueError("k has no heads: pass None")
     if inplace:
-        if _overlaps(q) or (k is not None and _overlaps(k)):
-            raise ValueError("inplace needs tensors whose values do not share memory (no expanded dimensions)")
         q_out, k_out = q, k
     else:
         q_out, k_out = torch.empty_like(q), None if k is None else torch.empty_like(k)
