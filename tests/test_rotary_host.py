@@ -61,3 +61,24 @@ def test_rotation_in_place_refuses_shared_values():
             rotary(q, k, pos, freq, inplace=True)
     with pytest.raises(RuntimeError, match="no CPU path"):  # into new tensors: inputs may share
         rotary(x, x, pos, freq)
+
+
+@pytest.mark.parametrize("base,original,rd,low,high", [
+    (10000.0, 65536, 128, 40, 65),    # the slowest pair still turns 1.2 times: the ramp ends behind it
+    (10000.0, 131072, 64, 22, 35),
+    (10000.0, 4096, 128, 20, 46),     # the ramp ends at pair 45.03, before the last one
+    (500000.0, 8192, 128, 18, 35),
+    (10.0, 10 ** 9, 8, 7, 7),         # every pair turns often: nothing is stretched
+])
+def test_yarn_ramp(base, original, rd, low, high):
+    """The ramp's ends, worked out by hand as rd ln(original / (2 pi turns)) / (2 ln base), rounded down for 32
+    turns and up for one, and kept within [0, rd - 1]; between them a linear share of f / factor."""
+    factor = 8.0
+    f = rotary_inv_freq(rd, base=base)[0]
+    got, _ = rotary_inv_freq(rd, base=base, scaling="yarn", factor=factor, original_max_position=original)
+    for i in range(rd // 2):
+        share = min(1.0, max(0.0, (i - low) / max(high - low, 1e-3)))
+        want = f[i].item() * (1 - share) + f[i].item() / factor * share
+        assert abs(got[i].item() - want) <= 1e-12 * want
+    turns = original * f / (2 * torch.pi)
+    assert (got[turns > 1.001] > f[turns > 1.001] / factor * (1 + 1e-9)).all()  # none of these is stretched all the way

@@ -25,8 +25,9 @@ def rotary_inv_freq(rotary_dim, base=10000.0, scaling=None, factor=1.0, original
     f_i = base^(-2 i / rotary_dim). Scalings for contexts `factor` times longer than
     original_max_position: "linear" f_i / factor; "ntk" base * factor^(rd / (rd - 2)), which leaves the
     fastest pair and divides the slowest by factor; "yarn" f_i where a pair turns more than beta_fast times
-    within original_max_position, f_i / factor where it turns less than beta_slow times, a linear
-    ramp over the pair's index between, and the magnitude 0.1 ln(factor) + 1.
+    within original_max_position, f_i / factor where it turns less than beta_slow times, between them a
+    linear ramp over the pair's index (from the pair at or before the one, to the pair at or behind the other,
+    within [0, rotary_dim - 1] as published), and the magnitude 0.1 ln(factor) + 1.
     """
     if scaling not in SCALINGS:
         raise ValueError(f"scaling must be one of {SCALINGS}, got {scaling!r}")
@@ -46,7 +47,8 @@ def rotary_inv_freq(rotary_dim, base=10000.0, scaling=None, factor=1.0, original
             return rotary_dim * math.log(original_max_position / (turns * 2 * math.pi)) / (2 * math.log(base))
 
         low = max(0, math.floor(pair_of(beta_fast)))
-        high = min(rotary_dim // 2 - 1, math.ceil(pair_of(beta_slow)))
+        # (The end may lie behind the last pair, which then still turns more than beta_slow times.)
+        high = min(rotary_dim - 1, math.ceil(pair_of(beta_slow)))
         stretched = ((i - low) / max(high - low, 1e-3)).clamp(0, 1)
         f = f * (1 - stretched) + f / factor * stretched
         magnitude = 0.1 * math.log(factor) + 1.0
