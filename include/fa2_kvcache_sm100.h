@@ -89,7 +89,8 @@ typedef struct Fa2RotaryParams {
  * cache_seqlens[b] counts them already. Fixed-length: k, v [B, H, N, D], n_b = seqlen; a sequence
  * with cache_seqlens[b] == 0 is skipped. Packed (cu_seqlens != NULL): k, v [total, H, D] with the
  * token axis as n, n_b = cu_seqlens[b + 1] - cu_seqlens[b]. Two positions written by one call must
- * not share a cache row (a page that two sequences share may be read, not appended to). */
+ * not share a cache row (a page that two sequences share may be read, not appended to). Sums that
+ * fall or go past seqlen are reported; a sequence that goes past it is left out. */
 typedef struct Fa2Kv8AppendParams {
   Fa2Kv8Cache cache;
   const void* k;
@@ -109,7 +110,8 @@ typedef struct Fa2Kv8AppendParams {
 
 /* Reads the first n_b keys of every sequence back into k_out, v_out [total, H, D] (contiguous),
  * n_b = cu_seqlens[b + 1] - cu_seqlens[b]. Rows past cu_seqlens[batch] are left as they were; rows
- * whose page is refused are zeros. */
+ * whose page is refused, and those of a sequence that goes past `total`, are zeros. Sums that fall or
+ * go past `total` are reported. */
 typedef struct Fa2Kv8ReadParams {
   Fa2Kv8Cache cache;
   void* k_out;

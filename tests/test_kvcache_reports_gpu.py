@@ -110,3 +110,44 @@ def test_a_refused_number_of_queries_leaves_the_others_alone(group, N_q):
             ref, weight, spread, small = serving.attention(q[cu[b]:cu[b + 1]], cache, bt[b:b + 1], sl[b:b + 1], cu_seqlens_q=alone)
             got, qs = out[cu[b]:cu[b + 1]], q[cu[b]:cu[b + 1]]
             assert ((got.double() - ref).abs() <= tolerance(qs, weight, spread, small, ref, 300, 8.0)).all()
+
+
+def test_append_and_read_report_sums_that_fall_or_leave_their_tensor():
+    """A sequence that goes past the tensor is left out (read: zeros where its rows are), the others are right;
+    sums that fall are reported. 200 sequences: more than a block's threads."""
+    lens = [3 + b % 5 for b in range(200)]
+    cache, bt, sl, cu, k, v = filled(lens, 16, 2, 64, seed=29)
+    total = int(cu[-1])
+    held = [t.view(torch.uint8).clone() if t.dtype == torch.float8_e4m3fn else t.clone() for t in cache]
+
+    def unchanged():
+        return all(torch.equal(torch.nan_to_num(t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t), torch.nan_to_num(h))
+                   for t, h in zip(cache, held))
+
+    kr, vr = kvcache.kvcache_read_fp8(cache, bt, cu, total)
+    check_device_errors()
+    short = total - 2  # the last sequence has three rows or more
+    kvcache.kvcache_append_fp8(k[:short] * 1.0, v[:short] * 1.0, cache, bt, sl, cu_seqlens=cu)
+    reported(_lib.FA2_ERR_SHAPE)
+    assert unchanged()  # the same rows again, and none of the last sequence's
+    changed = k.clone()
+    changed[int(cu[-2]):] += 1
+    kvcache.kvcache_append_fp8(changed[:short], v[:short], cache, bt, sl, cu_seqlens=cu)
+    reported(_lib.FA2_ERR_SHAPE)
+    assert unchanged()
+    ks, vs = kvcache.kvcache_read_fp8(cache, bt, cu, short)
+    reported(_lib.FA2_ERR_SHAPE)
+    at = int(cu[-2])
+    assert torch.equal(ks[:at], kr[:at]) and torch.equal(vs[:at], vr[:at])
+    assert (ks[at:] == 0).all() and (vs[at:] == 0).all()
+    for i in (1, 150, 199):
+        fallen = cu.clone()
+        fallen[i] = fallen[i + 1] + 1
+        kvcache.kvcache_read_fp8(cache, bt, fallen, total)
+        reported(_lib.FA2_ERR_SHAPE)
+        kvcache.kvcache_append_fp8(k[:total], v[:total], cache, bt, sl, cu_seqlens=fallen)
+        reported(_lib.FA2_ERR_SHAPE)
+    negative = cu.clone()
+    negative[0] = -1
+    kvcache.kvcache_read_fp8(cache, bt, negative, total)
+    reported(_lib.FA2_ERR_SHAPE)

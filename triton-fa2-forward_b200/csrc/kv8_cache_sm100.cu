@@ -182,10 +182,10 @@ __global__ void __launch_bounds__(128) append_kernel(const RowArgs a) {
       on = false;
       b = a.batch - 1;
     }
-    const int start = __ldg(a.cu + b);
-    n_new = __ldg(a.cu + b + 1) - start;
+    const int start = __ldg(a.cu + b), end = __ldg(a.cu + b + 1);
+    n_new = end - start;
     i = t - start;
-    if (i < 0) on = false;  // a row before the first sequence
+    if (i < 0 || end > a.n) on = false;  // a row before the first sequence; a sequence that goes past the tensor
   } else {
     b = tb;
     i = tn;
@@ -213,6 +213,7 @@ __global__ void __launch_bounds__(128) append_kernel(const RowArgs a) {
       if (part == 0) const_cast<float*>(z ? a.c.vs : a.c.ks)[scale_at(a.c, z != 0, page, row, h)] = scale;
     }
   }
+  if (a.cu != nullptr) check_sums(a.cu, a.batch, a.n, a.err);
 }
 
 template <int D, bool BF16>
@@ -225,13 +226,15 @@ __global__ void __launch_bounds__(128) read_kernel(const RowArgs a) {
   token_head(a, min(row_id, a.rows - 1), t, h);
   token_head(a, first, t0, h0);
   const int b = walk_sequence(a.cu, a.batch, block_first_sequence(a.cu, a.batch, t0), t);
+  check_sums(a.cu, a.batch, a.n, a.err);
   if (row_id >= a.rows || b >= a.batch) return;
   const int pos = t - __ldg(a.cu + b);
   if (pos < 0) return;
   int page = 0, row = 0;
   uint2 w[2][2] = {};
   float scale[2] = {};
-  if (find_row(a, b, pos, page, row)) {
+  const bool whole = __ldg(a.cu + b + 1) <= a.n;  // a sequence that goes past the tensor: zeros
+  if (find_row(a, b, pos, page, row) && whole) {
 #pragma unroll
     for (int z = 0; z < 2; ++z) {
       const uint8_t* src = (z ? a.c.v : a.c.k) + codes_at(a.c, z != 0, page, row, h) + part * 8;

@@ -138,6 +138,15 @@ __device__ __forceinline__ int walk_sequence(const int* cu, int batch, int b, in
   return b;
 }
 
+// Sums that fall, or go past the tensor's `total` rows, are reported, by the first block.
+__device__ __forceinline__ void check_sums(const int* cu, int batch, int total, int* err) {
+  if (blockIdx.x != 0) return;
+  for (int i = static_cast<int>(threadIdx.x); i < batch; i += static_cast<int>(blockDim.x)) {
+    const int from = __ldg(cu + i), to = __ldg(cu + i + 1);
+    if (from < 0 || to < from || to > total) report(err, FA2_ERR_SHAPE);
+  }
+}
+
 // n / d by a multiplication, 0 <= n < 2^31: hi(n mul) >> shift with mul = 2^(31 + s) / d + 1, d <= 2^s
 // (too large by less than n 2^-(31 + s) < 1 / d).
 struct Divisor {

@@ -162,7 +162,8 @@ def kvcache_append_fp8(k, v, cache, block_table, cache_seqlens, cu_seqlens=None)
 def kvcache_read_fp8(cache, block_table, cu_seqlens, total, dtype=torch.bfloat16):
     """The first n_b keys and values of every sequence, n_b = cu_seqlens[b + 1] - cu_seqlens[b], back in
     16 bits and packed as attention_varlen takes them: (k, v), each [total, H_kv, D]. Rows past
-    cu_seqlens[B] are not written; rows of a refused page are zeros. Asynchronous.
+    cu_seqlens[B] are not written; rows of a refused page, or of a sequence that goes past total, are zeros.
+    Asynchronous.
     """
     fields, shape, tensors = _cache_fields(cache)
     assert dtype in _DTYPES, "dtype must be fp16 or bf16"
