@@ -13,7 +13,8 @@
  *     scale = max|x| / 448,  code = e4m3(x / scale) (round to nearest even; a zero row: 0 and 0)
  * and stands for code * scale. A row that holds a NaN or an infinity is stored as codes 0 and a
  * NaN scale, so it reads back as NaN; no code written here is a NaN. Strides are free (page, row,
- * head) as long as every row of codes starts on a 16-byte boundary; pages whose rows of one head
+ * head) as long as every row of codes starts on a 16-byte boundary (and, to be written, the rows lie
+ * apart: the dimensions nest, no row is another's memory); pages whose rows of one head
  * are adjacent (head stride = page_size * head_dim) are read fastest.
  *
  * Sequence b's key j is in page block_table[b * block_table_stride + j / page_size], row

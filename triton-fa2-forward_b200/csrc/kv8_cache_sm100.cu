@@ -15,6 +15,9 @@
 
 #include "kv8_common.cuh"
 
+#include <algorithm>
+#include <utility>
+
 namespace {
 
 using namespace fa2kv;
@@ -285,6 +288,20 @@ int launch_read(const RowArgs& a, bool bf, cudaStream_t s) {
   return launch_status();
 }
 
+// Whether the rows of a cache tensor, `inner` values each, lie apart: sorted by stride, each dimension's
+// step is past all that the smaller ones span (as in every slice of a dense tensor).
+bool rows_apart(const Fa2Kv8Cache& c, const int64_t (&stride)[3], int64_t inner) {
+  std::pair<int64_t, int64_t> dims[3] = {{stride[0], c.num_pages}, {stride[1], c.page_size}, {stride[2], c.heads_kv}};
+  std::sort(dims, dims + 3);
+  int64_t span = inner;
+  for (const auto& [step, n] : dims) {
+    if (n <= 1) continue;
+    if (step < span) return false;
+    span += step * (n - 1);
+  }
+  return true;
+}
+
 bool vec_rows(const void* p, const int64_t st[4], int64_t nb, int64_t nh, int64_t nn) {
   return aligned16(p) && st[3] == 1 && (nb <= 1 || (st[0] & 7) == 0) && (nh <= 1 || (st[1] & 7) == 0) &&
          (nn <= 1 || (st[2] & 7) == 0);
@@ -312,6 +329,11 @@ int fa2_kv8_append_sm100_check(const Fa2Kv8AppendParams* p) {
   }
   const int rc = check_cache(p->cache);
   if (rc != FA2_OK) return rc;
+  const Fa2Kv8Cache& c = p->cache;
+  if (!rows_apart(c, c.k_stride, c.head_dim) || !rows_apart(c, c.v_stride, c.head_dim) || !rows_apart(c, c.ks_stride, 1) ||
+      !rows_apart(c, c.vs_stride, 1)) {
+    return FA2_ERR_LAYOUT;
+  }
   if (p->batch < 1 || p->seqlen < 0 || p->pages_per_seq < 1) return FA2_ERR_SHAPE;
   // Rows (tokens x heads) are counted in 31 bits.
   if (static_cast<int64_t>(p->cu_seqlens != nullptr ? 1 : p->batch) * p->seqlen > 0x7fff0000ll / p->cache.heads_kv) return FA2_ERR_SHAPE;
