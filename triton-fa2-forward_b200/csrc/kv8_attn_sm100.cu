@@ -105,7 +105,6 @@ __device__ __forceinline__ void decode_part(const AttnArgs& a, uint8_t* smem, co
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
   const int rows = sq.n_q * a.group;
-  constexpr int row0 = 0;
 
   const uint32_t ring = fa2::smem_u32(smem) + warp * C::RING;
   const int n_groups = (k1 - k0 + DEC_KEYS - 1) / DEC_KEYS;
@@ -115,10 +114,10 @@ __device__ __forceinline__ void decode_part(const AttnArgs& a, uint8_t* smem, co
   // of key `lane`.
   constexpr int STEP = 32 / C::PIECES;
   const int my_row = lane / C::PIECES, my_piece = lane % C::PIECES;
-  const uint8_t* kh = a.c.k + h * a.c.k_st[2] + my_piece * 16;
-  const uint8_t* vh = a.c.v + h * a.c.v_st[2] + my_piece * 16;
-  const float* ksh = a.c.ks + h * a.c.ks_st[2];
-  const float* vsh = a.c.vs + h * a.c.vs_st[2];
+  const uint8_t* kh = a.c.k + static_cast<int64_t>(h) * a.c.k_head + my_piece * 16;
+  const uint8_t* vh = a.c.v + static_cast<int64_t>(h) * a.c.v_head + my_piece * 16;
+  const float* ksh = a.c.ks + static_cast<int64_t>(h) * a.c.ks_head;
+  const float* vsh = a.c.vs + static_cast<int64_t>(h) * a.c.vs_head;
   auto group_pos = [&](int it) { return k0 + DEC_KEYS * (warp + DEC_WARPS * it); };
   // The next group's place: its page's index in the table, its first row there, and the page itself,
   // fetched one group ahead. Each half of a group, 16 keys, lies in one page; both do unless pages
@@ -206,12 +205,12 @@ __device__ __forceinline__ void decode_part(const AttnArgs& a, uint8_t* smem, co
   __shared__ float q_scale[DEC_WARPS][16];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    const int row = row0 + 8 * t + g;
+    const int row = 8 * t + g;
     constexpr int NB = D >= 64 ? 16 : D / 4;  // values of a contiguous piece
     uint32_t w[D / 8];                        // D / 4 values
     uint32_t top = 0;
     const bool in = row < rows;
-    const uint16_t* src = q_row(a, sq, b, h, in ? row : row0);
+    const uint16_t* src = q_row(a, sq, b, h, in ? row : 0);
 #pragma unroll
     for (int p = 0; p < D / 4 / NB; ++p) {
       const uint32_t* s = reinterpret_cast<const uint32_t*>(src + p * 64 + c * NB);
@@ -244,12 +243,12 @@ __device__ __forceinline__ void decode_part(const AttnArgs& a, uint8_t* smem, co
     for (int i = 0; i < 2; ++i) {
       const int r = 8 * t + 2 * c + i;
       row_sc[t][i] = q_scale[warp][r];
-      lim[t][i] = row0 + r < rows ? last_key(a, sq, query_of(a, row0 + r)) : -1;
+      lim[t][i] = r < rows ? last_key(a, sq, query_of(a, r)) : -1;
       m[t][i] = -INFINITY;
       l[t][i] = 0.0f;
     }
   }
-  const int lim_first = last_key(a, sq, query_of(a, row0));  // the smallest of the block's rows
+  const int lim_first = last_key(a, sq, query_of(a, 0));  // the smallest of the block's rows
 
   float o[NT][D / 16][4];
 #pragma unroll
@@ -461,8 +460,7 @@ __device__ __forceinline__ void decode_part(const AttnArgs& a, uint8_t* smem, co
   __syncthreads();
   constexpr int PARTS = DEC_WARPS * 32 / ROWS;  // threads of a row
   const int r = static_cast<int>(threadIdx.x) / PARTS, part = static_cast<int>(threadIdx.x) % PARTS;
-  const int row = row0 + r;
-  if (row >= rows) return;  // (no barrier follows in here)
+  if (r >= rows) return;  // (no barrier follows in here)
   float mx = -INFINITY;
 #pragma unroll
   for (int w = 0; w < DEC_WARPS; ++w) mx = fmaxf(mx, wm[w * 16 + r]);
@@ -475,7 +473,7 @@ __device__ __forceinline__ void decode_part(const AttnArgs& a, uint8_t* smem, co
     sum = f[w] == 0.0f ? sum : fmaf(f[w], lw, sum);
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  const int64_t part_row = static_cast<int64_t>(slot) * ROWS + row;
+  const int64_t part_row = static_cast<int64_t>(slot) * ROWS + r;
   constexpr int PER = D / PARTS > 0 ? (D / PARTS < 8 ? D / PARTS : 8) : 1;  // neighbouring columns at a time
   for (int d = part * PER; d < D; d += PARTS * PER) {
     float acc[PER] = {};
@@ -490,7 +488,7 @@ __device__ __forceinline__ void decode_part(const AttnArgs& a, uint8_t* smem, co
 #pragma unroll
       for (int j = 0; j < PER; ++j) a.o_part[part_row * D + d + j] = acc[j] * inv;
     } else {
-      uint16_t* dst = o_row(a, sq, b, h, row) + d;
+      uint16_t* dst = o_row(a, sq, b, h, r) + d;
       if constexpr (PER >= 2) {
 #pragma unroll
         for (int j = 0; j < PER; j += 2) {

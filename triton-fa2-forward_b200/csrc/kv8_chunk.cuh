@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
     while (next_piece(o)) {
       const int k0 = o.t0 * 128;
       const int* bt = a.bt + o.b * a.bt_stride;
-      const uint8_t* head = (is_v ? a.c.v + o.h * a.c.v_st[2] : a.c.k + o.h * a.c.k_st[2]) + my_piece * 16;
+      const uint8_t* head = (is_v ? a.c.v + static_cast<int64_t>(o.h) * a.c.v_head : a.c.k + static_cast<int64_t>(o.h) * a.c.k_head) + my_piece * 16;
       // Pages of a tile: lane l has the one of rows 16 l (or of them all). -1: none, or refused.
       auto page_for = [&](int n) -> int {
         const int key = k0 + n * 128 + 16 * lane;
@@ -393,8 +393,8 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
         const int key = k0 + n * 128 + tid, row = key - page_of(a.c, key) * a.c.page_size;
         sk = sv = 0.0f;
         if (page >= 0) {
-          sk = __ldg(a.c.ks + o.h * a.c.ks_st[2] + static_cast<int64_t>(page) * a.c.ks_page + static_cast<int64_t>(row) * a.c.ks_row);
-          sv = __ldg(a.c.vs + o.h * a.c.vs_st[2] + static_cast<int64_t>(page) * a.c.vs_page + static_cast<int64_t>(row) * a.c.vs_row);
+          sk = __ldg(a.c.ks + static_cast<int64_t>(o.h) * a.c.ks_head + static_cast<int64_t>(page) * a.c.ks_page + static_cast<int64_t>(row) * a.c.ks_row);
+          sv = __ldg(a.c.vs + static_cast<int64_t>(o.h) * a.c.vs_head + static_cast<int64_t>(page) * a.c.vs_page + static_cast<int64_t>(row) * a.c.vs_row);
         } else if (page == -2) {  // queries that see a key of a refused page get NaN
           sk = __uint_as_float(0x7fc00000u);
           report(a.err, FA2_ERR_PAGE);

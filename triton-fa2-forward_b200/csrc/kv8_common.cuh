@@ -20,11 +20,10 @@ struct Cache {
   const uint8_t* v;
   const float* ks;
   const float* vs;
-  int64_t k_st[3], v_st[3], ks_st[3], vs_st[3];  // (page, row, head)
   int num_pages, page_size, page_shift;           // shift >= 0 where page_size is a power of two
   int heads_kv;
-  // The same strides in 32 bits (page strides of codes in 16-byte units), for offsets that are one
-  // widening product each.
+  // Strides in 32 bits (page strides of codes in 16-byte units), for offsets that are one widening
+  // product each.
   int k_page16, v_page16, ks_page, vs_page, k_row, v_row, ks_row, vs_row, k_head, v_head, ks_head, vs_head;
 };
 
@@ -123,8 +122,8 @@ __device__ __forceinline__ uint16_t x1_of_float(float x) {
 
 // The sequence whose packed rows hold row `t`: the largest b with cu[b] <= t among b0.. (cu is
 // non-decreasing where it is right; where it is not, the caller's own range test refuses the row).
-// The block's first row is located by all its threads at once (one round of loads for 256
-// sequences), the others by walking on from there.
+// The block's first row is located by all its threads at once (one round of loads for as many
+// sequences as it has threads, 128 in the kernels here), the others by walking on from there.
 __device__ __forceinline__ int block_first_sequence(const int* cu, int batch, int t) {
   int n = 0;
   for (int base = 0; base < batch; base += static_cast<int>(blockDim.x)) {
@@ -206,12 +205,6 @@ inline Cache device_cache(const Fa2Kv8Cache& c) {
   d.v = static_cast<const uint8_t*>(c.v);
   d.ks = c.k_scale;
   d.vs = c.v_scale;
-  for (int i = 0; i < 3; ++i) {
-    d.k_st[i] = c.k_stride[i];
-    d.v_st[i] = c.v_stride[i];
-    d.ks_st[i] = c.ks_stride[i];
-    d.vs_st[i] = c.vs_stride[i];
-  }
   d.num_pages = c.num_pages;
   d.page_size = c.page_size;
   d.page_shift = -1;
