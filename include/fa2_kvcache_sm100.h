@@ -155,7 +155,7 @@ typedef struct Fa2Kv8AttnParams {
   int32_t heads_q;
   int32_t seqlen_q;     /* N, or the largest of a packed batch */
   int32_t total_q;      /* packed: rows of q and o */
-  int32_t max_seqlen_k; /* upper bound of cache_seqlens */
+  int32_t max_seqlen_k; /* upper bound of cache_seqlens (which is 2^31 - 1024 at most) */
   int32_t dtype;
   int32_t causal;
   int32_t causal_align;

@@ -187,5 +187,20 @@ int main() {
       ++bad;
     }
   }
+  // The longest sequence: its tiles, as many as there are, in shares that lie in order.
+  for (const int n_q : {1, 100}) {
+    Call c;
+    c.lens = {MAX_KEYS, 5};
+    c.finish(4, 1, n_q, 0, MAX_KEYS, 1, 1, 296);
+    if (!walk(c, true) || Line::tiles(c.a, sequence(c.a, 0), 0) != (1 << 24) - 8) {
+      std::printf("%d keys, %d queries\n", MAX_KEYS, n_q);
+      ++bad;
+    }
+    c.lens[0] = MAX_KEYS + 1;
+    if (sequence(c.a, 0).len != 0 || c.err != FA2_ERR_SHAPE) {
+      std::printf("a longer one is not refused\n");
+      ++bad;
+    }
+  }
   return bad ? 1 : 0;
 }

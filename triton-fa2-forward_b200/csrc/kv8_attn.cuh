@@ -5,9 +5,11 @@
 //     o_i  = sum_j (p_ij sv_j) cv_j / sum_j p_ij
 // The first product runs on fp16 operands for few rows (q' below 2^15, exact) and on 8-bit ones for
 // many (see there). The second runs on fp16: e4m3 codes are exact in it, and P' = p_ij sv_j
-// 2^(6 - e), with e the largest exponent of the sv seen so far, is rounded to it (relative error
-// 2^-11, below half a step of the output; P' < 2^15, and its range reaches 2^-30 below the row's
-// largest p). Sums, statistics and scales are fp32.
+// 2^(6 - e), with e the largest exponent of the sv seen so far, is rounded to it (2^-11 of each: an
+// eighth of half a bf16 step of the output; for fp16 as much as half a step, so such outputs are about 1.5 times
+// as far from the exact ones as their own rounding alone would put them, as with any 16-bit P; a second
+// term of P' would double this product). P' < 2^15, its range reaches 2^-30 below (p = 1, the largest
+// sv). Sums, statistics and scales are fp32.
 #pragma once
 
 #include "kv8_common.cuh"
@@ -39,6 +41,7 @@ struct AttnArgs {
 
 constexpr float RESCALE_TH = 8.0f;  // log2: the reference max moves when a row's max grows by more
 constexpr int P_SHIFT = 6;          // P' = p * sv * 2^(P_SHIFT - e), see above
+constexpr int MAX_KEYS = 0x7fffffff - 1023;  // of a sequence: positions a few tiles further fit 32 bits
 constexpr int EB_MIN = 8;           // smallest exponent field used for e (a multiplier stays finite)
 
 FA2_HOST_DEVICE int query_of(const AttnArgs& a, int row) { return divide(a.by_group, row); }

@@ -828,7 +828,7 @@ int fa2_kv8_attn_sm100(const Fa2Kv8AttnParams* p, void* stream) {
   a.heads_kv = p->cache.heads_kv;
   a.n_q = p->seqlen_q;
   a.total_q = p->total_q;
-  a.max_k = p->max_seqlen_k;
+  a.max_k = std::min(p->max_seqlen_k, MAX_KEYS);
   a.causal = p->causal;
   a.bottom_right = p->causal && p->causal_align == FA2_CAUSAL_BOTTOM_RIGHT;
   a.workers = r.workers;
