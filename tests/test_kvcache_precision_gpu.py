@@ -69,3 +69,64 @@ def test_each_kernel_within_its_own_bound(dtype, D, group, N_q):
         out, weight, spread, small = serving.attention(q, cache, bt, sl, causal=kw.get("causal", True))
         err, tol = (got.double() - out).abs(), bound(q, group * N_q, weight, spread, small, out, max(lens), 8.0)
         assert (err <= tol).all(), f"worst {(err / tol).max().item():.3f} of the tolerance, err {err.max().item():.3e}"
+
+
+def plain(q, cache, bt, n, sm_scale):
+    """One sequence's causal attention in 64 bits: (out, weight, spread, small, top), the first four as
+    oracle.serving.attention gives them but over the keys that have any weight (2^-100 of the row's sum), top the
+    largest p_ij max|v_j| / sum_j p_ij of a row: what a rounding of a product P V is relative to."""
+    k, v = (serving.rows_of(cache[i], cache[i + 2], bt, 0, n) for i in (0, 1))
+    H, N_q, D = q.shape[1:]
+    group = H // k.shape[1]
+    out, weight = torch.zeros(2, *q.shape, dtype=torch.float64, device="cuda")
+    spread, small, top = torch.zeros(3, *q.shape[:3], dtype=torch.float64, device="cuda")
+    sees = torch.ones(N_q, n, dtype=torch.bool, device="cuda").tril(n - N_q)
+    for h in range(H):
+        x, key, val = q[0, h].double(), k[:, h // group], v[:, h // group]
+        p = torch.softmax((x @ key.T * sm_scale).masked_fill(~sees, -torch.inf), -1)
+        p = torch.where(p < 2.0 ** -100, torch.zeros_like(p), p)
+        out[0, h], weight[0, h] = p @ val, p @ val.abs()
+        spread[0, h] = torch.where(p > 0, x.abs() @ key.abs().T * sm_scale, torch.zeros_like(p)).amax(-1)
+        small[0, h] = x.abs().amax(-1) * torch.where(p > 0, key.abs().sum(-1), torch.zeros_like(p)).amax(-1) * sm_scale
+        top[0, h] = (p * val.abs().amax(-1)).amax(-1)
+    return out, weight, spread, small, top
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("N_q", [1, 6, 40, 200])  # 2, 12, 80 and 400 rows a kv head
+@pytest.mark.parametrize("D", [128, 64, 16])
+@pytest.mark.parametrize("where", ["last", "unheeded", "first", "everywhere", "spread"])
+def test_values_far_above_the_others(dtype, N_q, D, where):
+    """Value rows up to the type's largest, which some queries do not see or give no weight: they leave those
+    queries' outputs as they are. A row of P' is rounded relative to its own largest product: 2^-31 of it and 2^-19
+    where the values' scales lie within 2^12 of one another (a common exponent); n keys."""
+    n = 900
+    cache, bt, sl, cu, k, v = filled([n], 32, 1, D, dtype, seed=50)
+    k, v = k[:n].clone(), v[:n].float()
+    most = 3e38 if dtype == torch.bfloat16 else 6e4
+    v *= 1e-3
+    q = randn(1, 2, N_q, D, dtype=dtype, seed=51)
+    q[..., 0] = 8
+    k[..., 0] = 0.1
+    if where == "last":  # seen by the last query alone
+        v[n - 1:] = v[n - 1:].sign() * most
+    elif where == "unheeded":  # scores far below the others'
+        v[[3, 500, 899]] *= most * 1e3 / 8
+        k[[3, 500, 899], :, 0] = -40 * D ** 0.5
+    elif where == "first":  # a tile of them, soon outweighed
+        v[:128] *= most * 1e3 / 8
+        k[:128, :, 0] = -40 * D ** 0.5
+    elif where == "everywhere":
+        v = v.sign() * most
+    else:  # sizes over the type's whole range
+        g = torch.Generator().manual_seed(52)
+        size = torch.rand(n, 1, 1, generator=g).cuda() * 2 - 1
+        v *= 1e3 * (2.0 ** (110 * size) if dtype == torch.bfloat16 else 2.0 ** (10 * size))
+    kvcache_append_fp8(k, v.clamp(-most, most).to(dtype), cache, bt, sl, cu_seqlens=cu)
+    scale = D ** -0.5
+    out, weight, spread, small, top = plain(q, cache, bt, n, scale)
+    for splits in (None, 1, 3):
+        got = attention_kvcache_fp8(q, cache, bt, sl, sm_scale=scale, num_splits=splits)
+        tol = bound(q, 2 * N_q, weight, spread, small, out, n, 0.0) + n * 2.0 ** -19 * top[..., None]
+        err = (got.double() - out).abs()
+        assert (err <= tol).all(), f"worst {(err / tol).nan_to_num(1e9).max().item():.3f} of the tolerance"

@@ -8,8 +8,13 @@
 // 2^(6 - e), with e the largest exponent of the sv seen so far, is rounded to it (2^-11 of each: an
 // eighth of half a bf16 step of the output; for fp16 as much as half a step, so such outputs are about 1.5 times
 // as far from the exact ones as their own rounding alone would put them, as with any 16-bit P; a second
-// term of P' would double this product). P' < 2^15, its range reaches 2^-30 below (p = 1, the largest
-// sv). Sums, statistics and scales are fp32.
+// term of P' would double this product). P' < 2^15. Sums, statistics and scales are fp32.
+//
+// One e for all rows is right as long as the sv lie within 2^WIDE of one another: then P' of a row's largest
+// product is 2^-6 or more and 2^-25, half of fp16's smallest step, is 2^-19 of that. Beyond, from the group
+// or tile of keys on where they first do, every row has an e of its own, that of its largest product p_ij
+// sv_j: a value row of 10^30 does not touch the queries that do not see it or give it no weight. Exponents of
+// a row also fall, with its sums, when its maximum grows.
 #pragma once
 
 #include "kv8_common.cuh"
@@ -42,7 +47,8 @@ struct AttnArgs {
 constexpr float RESCALE_TH = 8.0f;  // log2: the reference max moves when a row's max grows by more
 constexpr int P_SHIFT = 6;          // P' = p * sv * 2^(P_SHIFT - e), see above
 constexpr int MAX_KEYS = 0x7fffffff - 1023;  // of a sequence: positions a few tiles further fit 32 bits
-constexpr int EB_MIN = 8;           // smallest exponent field used for e (a multiplier stays finite)
+constexpr int EB_MIN = 16;          // smallest exponent field used for e (a multiplier stays finite)
+constexpr int WIDE = 12;            // log2: scales further apart than that give every row its own e, see above
 
 FA2_HOST_DEVICE int query_of(const AttnArgs& a, int row) { return divide(a.by_group, row); }
 
@@ -337,7 +343,23 @@ __host__ __device__ __forceinline__ bool pieces_together(Next next, Agree agree,
 __device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// Whether scales of which the smallest but zero is `low` (its bits - 1: a zero counts as the largest) and the
+// largest has the exponent field eb lie further apart than one unit for all rows takes.
+__device__ __forceinline__ bool too_wide(int eb, uint32_t low) { return low < (static_cast<uint32_t>(eb - WIDE) << 23) - 1u; }
+// A row's exponent from that of its largest new product (as a field, 0: none) and the one it had, and what its
+// sums are multiplied by; `alpha`: by what its maximum's growth scales them.
+__device__ __forceinline__ int row_unit(int product, int had, float alpha, float& factor) {
+  const int fall = 127 - static_cast<int>(__float_as_uint(alpha) >> 23);  // alpha <= 1; 127 for 0
+  const int e = max(max(EB_MIN, product), alpha > 0.0f ? had - fall : 0);
+  const int up = had - e;  // <= fall
+  factor = alpha > 0.0f && up >= -126 ? alpha * __uint_as_float(static_cast<uint32_t>(up + 127) << 23) : 0.0f;
+  return e;
+}
+
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }  // -126 <= e <= 127
+
+// The exponent of the power of two above a row's sum (0 and NaN: any, the row's O is 0 or NaN).
+__device__ __forceinline__ int above(float sum) { return min(static_cast<int>(__float_as_uint(sum) >> 23), 253) - 126; }
 
 // Exponent e such that a row with largest magnitude `top` (bits) times 2^(14 - e) stays below 2^15.
 __device__ __forceinline__ int row_exponent(uint32_t top_bits) {

@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace {
 
@@ -259,10 +260,14 @@ __device__ __forceinline__ void decode_part(const AttnArgs& a, uint8_t* smem, co
       for (int i = 0; i < 4; ++i) o[t][j][i] = 0.0f;
     }
   }
-  int eb = EB_MIN;  // exponent field of the largest finite sv so far
+  int eb = EB_MIN;  // exponent field of the largest finite sv so far ...
+  uint32_t low = 0xffffffffu;  // ... and the smallest but zero that this lane has met, its bits - 1
+  int er[NT][2];  // the rows' exponents, of their own once those are too far apart
   constexpr int HALVES = DEC_KEYS / 16;
 
-  for (int it = 0; it < mine; ++it) {
+  // A group of keys. `wide`: rows have exponents of their own. False (and nothing is done) where they should.
+  auto group = [&](auto is_wide, int it) -> bool {
+    constexpr bool wide = decltype(is_wide)::value;
     cp_async_wait<DEC_STAGES - 1>();
     __syncwarp();
     const uint32_t st = ring + (it % DEC_STAGES) * C::STAGE;
@@ -306,6 +311,7 @@ __device__ __forceinline__ void decode_part(const AttnArgs& a, uint8_t* smem, co
         lds<4>(st + 2 * C::CODES + (DEC_KEYS + 16 * z + 8 * y + g) * 4, &w);
         sv[z][y] = __uint_as_float(w);
         top = max(top, w & 0x7fffffffu);
+        low = min(low, (w & 0x7fffffffu) - 1u);
       }
     }
     top = __reduce_max_sync(0xffffffffu, top);
@@ -328,7 +334,7 @@ __device__ __forceinline__ void decode_part(const AttnArgs& a, uint8_t* smem, co
     }
     const bool masked = pos0 + DEC_KEYS - 1 > lim_first;
     const int eb_new = max(eb, static_cast<int>(top >> 23));  // the same in every lane
-    bool bump = eb_new > eb;
+    bool bump = !wide && (eb_new > eb || too_wide(eb_new, low));
     float cand[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -352,51 +358,93 @@ __device__ __forceinline__ void decode_part(const AttnArgs& a, uint8_t* smem, co
 #pragma unroll
         for (int z = 1; z < HALVES; ++z) v = fa2::fmax3(v, s[t][z][i], s[t][z][i + 2]);
         cand[t][i] = keys_max(v) * row_sc[t][i];
-        bump = bump || cand[t][i] > m[t][i] + RESCALE_TH;
+        if constexpr (!wide) bump = bump || cand[t][i] > m[t][i] + RESCALE_TH;
       }
     }
-    if (__any_sync(0xffffffffu, bump)) {
-      const float fe = eb_new - eb > 126 ? 0.0f : pow2f(eb - eb_new);
+    uint32_t pb[NT][HALVES][2];
+    if constexpr (!wide) {
+      if (__any_sync(0xffffffffu, bump)) {
+        if (__any_sync(0xffffffffu, too_wide(eb_new, low))) return false;
+        const float fe = eb_new - eb > 126 ? 0.0f : pow2f(eb - eb_new);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          float al[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            al[i] = 1.0f;
+            if (cand[t][i] > m[t][i] + RESCALE_TH) {
+              al[i] = fa2::ex2_mufu(m[t][i] - cand[t][i]);  // 0 the first time (m = -inf)
+              m[t][i] = cand[t][i];
+            }
+            l[t][i] *= al[i];
+            al[i] *= fe;
+          }
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[t][j][i] *= al[i & 1];
+          }
+        }
+        eb = eb_new;
+      }
+      const float gs = __uint_as_float(static_cast<uint32_t>(254 + P_SHIFT - eb) << 23);
+#pragma unroll
+      for (int z = 0; z < HALVES; ++z) {
+        sv[z][0] *= gs;
+        sv[z][1] *= gs;
+      }
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        float al[2];
+        const float m0 = m[t][0] == -INFINITY ? 0.0f : m[t][0], m1 = m[t][1] == -INFINITY ? 0.0f : m[t][1];
+#pragma unroll
+        for (int z = 0; z < HALVES; ++z) {
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const float p0 = fa2::ex2_mufu(fmaf(s[t][z][2 * y], row_sc[t][0], -m0));
+            const float p1 = fa2::ex2_mufu(fmaf(s[t][z][2 * y + 1], row_sc[t][1], -m1));
+            l[t][0] += p0;
+            l[t][1] += p1;
+            pb[t][z][y] = transpose8x8(x2_of_floats<false>(p0 * sv[z][y], p1 * sv[z][y]));
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float gs[2], f[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          al[i] = 1.0f;
+          float al = 1.0f, most = 0.0f;
           if (cand[t][i] > m[t][i] + RESCALE_TH) {
-            al[i] = fa2::ex2_mufu(m[t][i] - cand[t][i]);  // 0 the first time (m = -inf)
+            al = fa2::ex2_mufu(m[t][i] - cand[t][i]);
             m[t][i] = cand[t][i];
           }
-          l[t][i] *= al[i];
-          al[i] *= fe;
+          l[t][i] *= al;
+          const float mi = m[t][i] == -INFINITY ? 0.0f : m[t][i];
+#pragma unroll
+          for (int z = 0; z < HALVES; ++z) {
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const float p = fa2::ex2_mufu(fmaf(s[t][z][2 * y + i], row_sc[t][i], -mi));
+              l[t][i] += p;
+              s[t][z][2 * y + i] = p * sv[z][y];
+              most = fmaxf(most, fabsf(s[t][z][2 * y + i]));
+            }
+          }
+          er[t][i] = row_unit(static_cast<int>(__float_as_uint(keys_max(most)) >> 23), er[t][i], al, f[i]);
+          gs[i] = __uint_as_float(static_cast<uint32_t>(254 + P_SHIFT - er[t][i]) << 23);
+        }
+#pragma unroll
+        for (int z = 0; z < HALVES; ++z) {
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            pb[t][z][y] = transpose8x8(x2_of_floats<false>(s[t][z][2 * y] * gs[0], s[t][z][2 * y + 1] * gs[1]));
+          }
         }
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[t][j][i] *= al[i & 1];
-        }
-      }
-      eb = eb_new;
-    }
-    const float gs = __uint_as_float(static_cast<uint32_t>(254 + P_SHIFT - eb) << 23);
-    uint32_t pb[NT][HALVES][2];
-#pragma unroll
-    for (int z = 0; z < HALVES; ++z) {
-      sv[z][0] *= gs;
-      sv[z][1] *= gs;
-    }
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const float m0 = m[t][0] == -INFINITY ? 0.0f : m[t][0], m1 = m[t][1] == -INFINITY ? 0.0f : m[t][1];
-#pragma unroll
-      for (int z = 0; z < HALVES; ++z) {
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const float p0 = fa2::ex2_mufu(fmaf(s[t][z][2 * y], row_sc[t][0], -m0));
-          const float p1 = fa2::ex2_mufu(fmaf(s[t][z][2 * y + 1], row_sc[t][1], -m1));
-          l[t][0] += p0;
-          l[t][1] += p1;
-          pb[t][z][y] = transpose8x8(x2_of_floats<false>(p0 * sv[z][y], p1 * sv[z][y]));
+          for (int i = 0; i < 4; ++i) o[t][j][i] *= f[i & 1];
         }
       }
     }
@@ -428,18 +476,21 @@ __device__ __forceinline__ void decode_part(const AttnArgs& a, uint8_t* smem, co
     }
     __syncwarp();  // every lane has read the stage before it is filled again
     issue(it + DEC_STAGES);
-  }
+    return true;
+  };
+  int it = 0;
+  while (it < mine && group(std::false_type{}, it)) ++it;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) er[t][0] = er[t][1] = eb;
+  for (; it < mine; ++it) group(std::true_type{}, it);
   cp_async_wait<0>();
   __syncwarp();
 
-  // Merge the warps: (m, l, O) of each in shared memory, O in the sv's own units. Rows of O are D + 4
-  // floats apart: the four rows that the lanes of one g write lie in different banks.
+  // Merge the warps: (m, l, O / 2^above(l)) of each in shared memory. Rows of O are D + 4 floats apart: the four rows
+  // that the lanes of one g write lie in different banks.
   float* wo = reinterpret_cast<float*>(smem + warp * C::RING);
   float* wm = reinterpret_cast<float*>(smem + DEC_WARPS * C::RING);  // [warp][16]
   float* wl = wm + DEC_WARPS * 16;
-  // 2^(eb - 127 - P_SHIFT), as two factors so that neither leaves the normal range.
-  const int ex = eb - 127 - P_SHIFT;
-  const float u0 = pow2f(ex / 2), u1 = pow2f(ex - ex / 2);
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -450,6 +501,10 @@ __device__ __forceinline__ void decode_part(const AttnArgs& a, uint8_t* smem, co
         wm[warp * 16 + r] = m[t][i];
         wl[warp * 16 + r] = sum;
       }
+      // Out of the unit 2^(e - 127 - P_SHIFT), as two factors so that neither leaves the normal range, and over
+      // the power of two above the sum: an average of the values stays in range where a sum may not.
+      const int ex = er[t][i] - 127 - P_SHIFT - above(sum);
+      const float u0 = pow2f(ex / 2), u1 = pow2f(ex - ex / 2);
       float* dst = wo + r * (D + 4) + g * (D / 8);
 #pragma unroll
       for (int j = 0; j < D / 16; ++j) {
@@ -473,6 +528,8 @@ __device__ __forceinline__ void decode_part(const AttnArgs& a, uint8_t* smem, co
     sum = f[w] == 0.0f ? sum : fmaf(f[w], lw, sum);
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+  for (int w = 0; w < DEC_WARPS; ++w) f[w] = f[w] == 0.0f ? 0.0f : f[w] * pow2f(above(wl[w * 16 + r])) * inv;
   const int64_t part_row = static_cast<int64_t>(slot) * ROWS + r;
   constexpr int PER = D / PARTS > 0 ? (D / PARTS < 8 ? D / PARTS : 8) : 1;  // neighbouring columns at a time
   for (int d = part * PER; d < D; d += PARTS * PER) {
@@ -486,16 +543,16 @@ __device__ __forceinline__ void decode_part(const AttnArgs& a, uint8_t* smem, co
     }
     if (slot >= 0) {
 #pragma unroll
-      for (int j = 0; j < PER; ++j) a.o_part[part_row * D + d + j] = acc[j] * inv;
+      for (int j = 0; j < PER; ++j) a.o_part[part_row * D + d + j] = acc[j];
     } else {
       uint16_t* dst = o_row(a, sq, b, h, r) + d;
       if constexpr (PER >= 2) {
 #pragma unroll
         for (int j = 0; j < PER; j += 2) {
-          *reinterpret_cast<uint32_t*>(dst + j) = x2_of_floats<BF16>(acc[j] * inv, acc[j + 1] * inv);
+          *reinterpret_cast<uint32_t*>(dst + j) = x2_of_floats<BF16>(acc[j], acc[j + 1]);
         }
       } else {
-        dst[0] = x1_of_float<BF16>(acc[0] * inv);
+        dst[0] = x1_of_float<BF16>(acc[0]);
       }
     }
   }
@@ -612,12 +669,14 @@ __global__ void __launch_bounds__(128) merge_kernel(const AttnArgs a) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], o));
   }
+  // 2^-j <= 1 / n_parts on every weight: the sum of the parts stays in range as its average does.
+  const float down = pow2f(-(32 - __clz(cut.n_parts - 1)));
   for (int i0 = 0; i0 < cut.n_parts; i0 += 32) {
     float f[R];
 #pragma unroll
     for (int k = 0; k < R; ++k) {
       const float v = i0 + lane < cut.n_parts && r0 + 4 * k < rows ? a.lse_part[part(i0 + lane, r0 + 4 * k)] : -INFINITY;
-      f[k] = v == -INFINITY ? 0.0f : exp2f(v - (mx[k] == -INFINITY ? 0.0f : mx[k]));  // a NaN stays one
+      f[k] = v == -INFINITY ? 0.0f : exp2f(v - (mx[k] == -INFINITY ? 0.0f : mx[k])) * down;  // a NaN stays one
     }
     const int n = min(32, cut.n_parts - i0);
     constexpr int AT_ONCE = R == 1 ? 8 : 2;

@@ -27,7 +27,9 @@
 // bf16 queries fold them into that conversion (code * s_j in fp16, one rounding of at most 2^-11, an
 // eighth of the output's half step); for fp16 queries, whose half step is 2^-11 itself, the codes
 // stay exact and each probability is multiplied by its key's scale in fp32. K's scales multiply the
-// scores.
+// scores. From the tile on where a piece's value scales lie more than 2^WIDE apart, nothing is folded and
+// rows have exponents of their own (kv8_attn.cuh). That costs ordinary tiles up to 2% (the chunks above with
+// heads of 64 dims: 245 to 250 us, of 128: 300 to 301).
 //
 // Warps 0-3 / 4-7: softmax of tile 0 / 1, one thread a row (scores and P' live in TMEM, P' feeds the
 // second product from there). Warps 8-11: convert V. Warp 12: issues the products. Warps 13 and 14:
@@ -76,9 +78,9 @@ struct Ch {
   static constexpr int OFF_V = OFF_K + KSLOTS * CODES;
   static constexpr int OFF_RAW = OFF_V + CH_VSLOTS * VTILE;
   static constexpr int OFF_SC = OFF_RAW + RAW * CODES;          // [entry][2][128] words
-  static constexpr int OFF_HEAD = OFF_SC + CH_ENTRIES * 1024;   // [entry] exponent field of sv
-  static constexpr int OFF_MAX = OFF_HEAD + CH_ENTRIES * 4;     // [2][4 warps]
-  static constexpr int OFF_ML = OFF_MAX + 32;                   // [2][128]: tile 1's max and sum, for the merge
+  static constexpr int OFF_HEAD = OFF_SC + CH_ENTRIES * 1024;   // [entry] exponent field of sv, or -1: each row its own
+  static constexpr int OFF_MAX = OFF_HEAD + CH_ENTRIES * 4;     // [2][4 warps] largest and smallest sv
+  static constexpr int OFF_ML = OFF_MAX + 64;                   // [2][128]: tile 1's max and sum, for the merge
   static constexpr int OFF_QS = OFF_ML + 1024;                  // [2][128]: the rows' score factors
   static constexpr int OFF_PIECE = OFF_QS + 1024;               // [piece] 12 words
   static constexpr int OFF_BAR = OFF_PIECE + CH_PIECES * 48;
@@ -162,6 +164,12 @@ __device__ __forceinline__ bool conv_sync(bool ok) {
       "bar.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
       : "+r"(bad)::"memory");
   return bad == 0;
+}
+
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(v[0]), "r"(v[1]),
+               "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 
 template <int D, bool BF16>
@@ -400,7 +408,9 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
           report(a.err, FA2_ERR_PAGE);
         }
       };
-      int eb = EB_MIN;  // exponent field of the largest finite sv so far
+      int eb = EB_MIN;  // exponent field of the largest finite sv so far ...
+      uint32_t low = 0xffffffffu;  // ... and the smallest but zero, its bits - 1
+      bool wide = false;  // too far apart: from here on rows have exponents of their own, and V is not folded
       fetch_scales(0, page_for(0));
       int page = page_for(1);
 #pragma unroll 1
@@ -413,16 +423,25 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
           sk = __uint_as_float(0x7fc00000u);
           sv = 0.0f;
         }
-        const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(sv) & 0x7fffffffu);
-        volatile uint32_t* wm = reinterpret_cast<volatile uint32_t*>(smem + C::OFF_MAX) + (u & 1) * 4;
-        if (lane == 0) wm[warp - CH_CONV_WARP] = top;
+        const uint32_t bits = __float_as_uint(sv) & 0x7fffffffu;
+        const uint32_t top = __reduce_max_sync(0xffffffffu, bits), least = __reduce_min_sync(0xffffffffu, bits - 1u);
+        const uint32_t wm = sbase + C::OFF_MAX + (u & 1) * 32;
+        if (lane == 0) {
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(wm + (warp - CH_CONV_WARP) * 4), "r"(top) : "memory");
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(wm + 16 + (warp - CH_CONV_WARP) * 4), "r"(least) : "memory");
+        }
         conv_sync(true);
-        eb = max(eb, static_cast<int>(max(max(wm[0], wm[1]), max(wm[2], wm[3])) >> 23));
+        uint32_t tops[4], lows[4];
+        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(tops[0]), "=r"(tops[1]), "=r"(tops[2]), "=r"(tops[3]) : "r"(wm) : "memory");
+        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(lows[0]), "=r"(lows[1]), "=r"(lows[2]), "=r"(lows[3]) : "r"(wm + 16) : "memory");
+        eb = max(eb, static_cast<int>(max(max(tops[0], tops[1]), max(tops[2], tops[3])) >> 23));
+        low = min(low, min(min(lows[0], lows[1]), min(lows[2], lows[3])));
+        wide = wide || too_wide(eb, low);
         const float fv = __uint_as_float(static_cast<uint32_t>(254 + FOLD_SHIFT - eb) << 23);
         uint32_t* entry = reinterpret_cast<uint32_t*>(smem + C::OFF_SC) + en * 256;
         entry[tid] = __float_as_uint(sk);
-        entry[128 + tid] = FOLD ? split_scale(sv * fv) : __float_as_uint(sv * fv);
-        if (tid == 0) reinterpret_cast<int*>(smem + C::OFF_HEAD)[en] = eb;
+        entry[128 + tid] = wide ? __float_as_uint(sv) : FOLD ? split_scale(sv * fv) : __float_as_uint(sv * fv);
+        if (tid == 0) reinterpret_cast<int*>(smem + C::OFF_HEAD)[en] = wide ? -1 : eb;
         mbar_arrive(bar(CB_SC + en));
         fetch_scales(n + 1, page);  // on their way while V is converted
         page = page_for(n + 2);
@@ -444,7 +463,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
             y[2 * j + 1] = f16x2_of_e4m3x2(static_cast<uint16_t>(c[j] >> 16));
           }
           if constexpr (FOLD) {
-            const uint32_t ws = vsc[it * V_ROWS];
+            const uint32_t ws = wide ? 0x3c00u : vsc[it * V_ROWS];  // (one: the codes as they are)
             const uint32_t hi = __byte_perm(ws, ws, 0x1010), lo = __byte_perm(ws, ws, 0x3232);
 #pragma unroll
             for (int j = 0; j < 8; ++j) y[j] = hfma2(y[j], hi, hmul2(y[j], lo));
@@ -695,10 +714,9 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
           m = cand;
         }
         l *= alpha;
-        if (done > 0 && __any_sync(0xffffffffu, bump || eb_new > eb)) {
-          // (PV of the step before has retired: this step's scores were committed after it.)
-          alpha *= eb_new - eb > 126 ? 0.0f : pow2f(eb - eb_new);
-          const uint64_t a2 = fa2::f2_pack(alpha, alpha);
+        // O times a factor. (PV of the step before has retired: this step's scores were committed after it.)
+        auto scale_o = [&](float f) {
+          const uint64_t a2 = fa2::f2_pack(f, f);
 #pragma unroll 1
           for (int c = 0; c < D / 16; ++c) {
             uint32_t y[16];
@@ -715,9 +733,59 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
             fa2::tmem_st16(tO + c * 16, y);
           }
           fa2::tmem_wait_st();
+        };
+        const float mr = m == -INFINITY ? 0.0f : m;  // a row that has seen no key yet: p = 0, not NaN
+        if (__builtin_expect(eb_new < 0, 0)) {
+          // The row's own exponent: products p sv (2^-8 of them: p reaches 2^14) take the scores' place, then P'
+          // takes theirs, each 16 columns at a time (rare: small code, no registers kept).
+          float sum = 0.0f, most = 0.0f;
+#pragma unroll 1
+          for (int c = 0; c < 128; c += 16) {
+            uint32_t y[16];
+            fa2::tmem_ld16(tS + c, y);
+            fa2::tmem_wait_ld();
+            fa2::reg_fence16(y);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              uint32_t k, v;
+              asm volatile("ld.shared.b32 %0, [%1];" : "=r"(k) : "r"(sc_addr + (c + i) * 4));
+              asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(sc_addr + 512 + (c + i) * 4));
+              const float x = masked && c + i > lim ? -INFINITY : __uint_as_float(y[i]) * __uint_as_float(k);
+              const float p = fa2::ex2_mufu(fmaf(x, row_sc, -mr));
+              sum += p;
+              const float z = p * 0x1p-8f * __uint_as_float(v);
+              most = fmaxf(most, fabsf(z));
+              y[i] = __float_as_uint(z);
+            }
+            fa2::tmem_st16(tS + c, y);
+          }
+          fa2::tmem_wait_st();
+          l += sum;
+          const int product = static_cast<int>(__float_as_uint(most) >> 23);
+          float factor;
+          eb = row_unit(product > 0 ? product + 8 : 0, eb, alpha, factor);
+          if (done > 0 && __any_sync(0xffffffffu, factor != 1.0f)) scale_o(factor);
+          const float gs = __uint_as_float(static_cast<uint32_t>(254 + FOLD_SHIFT + 8 - eb) << 23);
+#pragma unroll 1
+          for (int c = 0; c < 64; c += 8) {
+            uint32_t y[16], pk[8];
+            fa2::tmem_ld16(tS + 2 * c, y);
+            fa2::tmem_wait_ld();
+            fa2::reg_fence16(y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) pk[i] = x2_of_floats<false>(__uint_as_float(y[2 * i]) * gs, __uint_as_float(y[2 * i + 1]) * gs);
+            tmem_st8(tS + c, pk);
+          }
+          fa2::tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(bar(CB_P + t));
+          mbar_arrive(bar(CB_PL + t));
+          continue;
+        }
+        if (done > 0 && __any_sync(0xffffffffu, bump || eb_new > eb)) {
+          scale_o(alpha * (eb_new - eb > 126 ? 0.0f : pow2f(eb - eb_new)));
         }
         eb = eb_new;
-        const float mr = m == -INFINITY ? 0.0f : m;  // a row that has seen no key yet: p = 0, not NaN
         const uint64_t sc2 = fa2::f2_pack(row_sc, row_sc), nm2 = fa2::f2_pack(-mr, -mr);
         uint64_t sum2[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -759,13 +827,14 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
         fa2::f2_unpack(fa2::f2_add(fa2::f2_add(sum2[0], sum2[1]), fa2::f2_add(sum2[2], sum2[3])), s0, s1);
         l += s0 + s1;
       }
-      // O, in the units of the last exponent: * 2^(eb - 127 - shift).
+      // O, in the units of the last exponent: * 2^(eb - 127 - shift), over the power of two above the sum: an
+      // average of the values stays in range where a sum may not.
       if (ok && done > 0) {
         ok = wait_warp(CB_O + t, o_at & 1u);
         ++o_at;
       }
       tc_fence_after();
-      const int ex = eb - 127 - FOLD_SHIFT;
+      const int ex = eb - 127 - FOLD_SHIFT - above(l);
       const float u0 = pow2f(ex / 2), u1 = pow2f(ex - ex / 2);
       float4* area = reinterpret_cast<float4*>(smem + C::OFF_Q + C::TERMS * C::CODES);  // [COLS / 4][128]
       float* ml = reinterpret_cast<float*>(smem + C::OFF_ML);
@@ -813,10 +882,11 @@ __global__ void __launch_bounds__(CH_THREADS, 1) chunk_kernel(const AttnArgs a) 
             f0 = m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : exp2f(m - mx);
             f1 = m1 == -INFINITY ? (l1 == 0.0f ? 0.0f : 1.0f) : exp2f(m1 - mx);
             sum = (f0 == 0.0f ? 0.0f : f0 * l) + (f1 == 0.0f ? 0.0f : f1 * l1);
+            f1 *= pow2f(above(l1));
           }
           inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         }
-        const float g0 = f0 * inv, g1 = f1 * inv;
+        const float g0 = f0 * inv * pow2f(above(l)), g1 = f1 * inv;
         // The warp's 32 rows go through where its rows of Q were, which are done with, so that rows are
         // stored in whole lines: 32 columns a term, 16-byte parts xor-ed with the row's number.
         uint8_t* stage = smem + C::OFF_Q + t * C::TERMS * C::CODES + q * 32 * 128;
