@@ -21,9 +21,10 @@ using namespace fa2kv;
 // between warps) and keeps its own running max, sum and output; the four warps are merged once at
 // the end. A 128-row tile would be 1/16 full and the way through shared memory and TMEM would cost
 // more than the bytes. (Warp-wide e4m3 products in place of conversions and fp16 ones were slower, 162
-// against 137 us at the time.) Measured: 4 sequences of 65536 keys, 8 kv heads of 128, one token, 554 MB,
-// 91 us (6.1 TB/s, 0.93 of the copy rate); one of 700 keys 11 us, most of it two launches and the way
-// to the first key; 48 of up to 8192 keys, 2 kv heads of 64, 54 MB, 27 us.
+// against 137 us at the time.) Measured in a graph: 4 sequences of 65536 keys, 8 kv heads of 128, one token,
+// 554 MB, 92 us (6.0 TB/s, 0.92 of the copy rate), 16 rows in place of 4 113 us; one of 700 keys 11.6 us,
+// most of it two launches and the way to the first key; 48 of up to 8192 keys, 2 kv heads of 64, 54 MB, 28 us.
+// Ordinary calls of these: 96, 24 (the host's) and 29 us.
 //
 // Operand layouts, lane (g, c) = (lane / 4, lane % 4). The products sum over d (QK^T) and over keys
 // (PV) in any order, so both operands use the order in which a lane's bytes lie in memory: for QK^T
@@ -36,8 +37,9 @@ constexpr int DEC_WARPS = 4;
 constexpr int DEC_KEYS = 32;   // of a group
 constexpr int DEC_STAGES = 2;  // 12 warps an SM x one group on its way: 96 KB
 constexpr int DEC_CTAS = 3;    // an SM at most
-// CTAs an SM that the work is shared among: two, three where rows of codes are shorter (4 sequences of
-// 65536 keys, D = 128: 91 and 96 us; 48 of up to 8192, D = 64: 30 and 27 us).
+// CTAs an SM that the work is shared among: two, three where rows of codes are shorter. Two / three for 4
+// sequences of 65536 keys and 8 kv heads: 128 dims 91 / 98 us, 64 59 / 55, 32 49 / 44, 16 46 / 40; for 48 of up
+// to 8192 and 2 kv heads 38.5 / 37, 30 / 28, 25 / 23, 22.6 / 21; the same in fp16.
 constexpr int dec_shares(int head_dim) { return head_dim > 64 ? 2 : 3; }
 
 template <int D>
@@ -739,8 +741,10 @@ Plan plan(const Fa2Kv8AttnParams* p) {
     // With fewer (sequence, head, block)s than that a multiple of their number cuts equal ones alike.
     const int64_t alike = most / units * units;
     if (r.block < 256) {
-      // Three tiles a share at least (8 heads of 8192 keys: 15 us with three or four, 16 with two, 18
-      // with fewer).
+      // Three tiles a share at least: more shares cost their finding and merging, fewer their keys. Us for 8
+      // heads of one sequence with one, two, three and more tiles a share: 700 keys 10.3, 11.0, 11.7, 12.3 (6
+      // tiles); 2000 keys 12.3, 11.6, 12.3, 12.3 (4), 14.4 (6); 8192 keys 17 (2), 16.4 (3), 14.6 (4), 15.8 (6),
+      // 16.4 (8), 19 (11). Short sequences would take one or two, long ones four.
       const int64_t least = std::max<int64_t>(3, (per_unit + most / units - 1) / (most / units));
       w = std::max<int64_t>(1, (per_unit + least - 1) / least) * units;
     } else {

@@ -8,7 +8,7 @@
 // the key's and the value's row of the same token and head: they share the page, and four loads are
 // in flight. Heads run fastest, as the packed tokens have them in memory.
 //
-// Measured: append of 17,000 tokens of 8 heads of 128, 103 MB, 25 us (4.1 TB/s, 0.62 of the copy
+// Measured in a graph: append of 17,000 tokens of 8 heads of 128, 103 MB, 26 us (4.0 TB/s, 0.61 of the copy
 // rate): the way from the sums over the table to the page lies before the stores, and a row costs
 // some 300 instructions a lane for its maximum, quotients and codes (with divisions 39 us). Read of
 // 157,000 tokens, 471 MB, 76 us (6.2 TB/s, 0.95); two or four rows a thread were no faster.

@@ -1,11 +1,13 @@
 // Attention over the 8-bit paged cache for many rows (chunks of prompts): tcgen05 products.
 //
 // The floor is the tensor cores' (4 D operations a score). What sets the step is a row tile's chain of
-// scores, softmax, PV and the next scores, which the other tile fills in part: tensor pipe 46%, issue
+// scores, softmax, PV and the next scores, which the other tile fills in part: tensor pipe 45%, issue
 // slots 49% and exponentials 47% busy, none of them full. Longer chains cost at once: an eighth of the
-// exponentials on the FMA pipe made it 5% slower. Measured: 2 chunks of
-// 512 tokens over 16384 keys, 32 heads of 128 over 8, 271 GFLOP, 287 us (943 TFLOP/s, 0.57 of the
-// bf16 peak); a step of 256 rows and 128 keys takes 2.35 us, a piece of work 10 us beside its steps.
+// exponentials on the FMA pipe made it 5% slower. Measured: 2 chunks of 512 tokens over 16384 keys, 32
+// heads of 128 over 8, 271 GFLOP, 289 us in short runs of a graph (938 TFLOP/s, 0.57 of the bf16 peak), 318 us
+// as ordinary calls in a row (850 TFLOP/s, at lower clocks), in fp16 350 us (a third operand of Q, shorter
+// rings); 20 rows a kv head in place of 2048 51 us, of which the bytes are 11. A step of 256 rows and 128 keys
+// takes 2.35 us, a piece of work 10 us beside its steps.
 //
 // A CTA owns 256 rows (queries x heads of a group) as two 128-row tiles that take turns: while one
 // tile's scores go through the softmax, the tensor core works on the other. With 128 rows or fewer both tiles hold the same rows and take
